@@ -111,6 +111,8 @@ EXPORTS = ("dg_rasterize_forward", "dg_rasterize_backward", "dg_rasterize_count"
            "dg_ring_upload", "dg_ring_pending", "dg_ring_destroy", "dg_image_u8_to_chw", "dg_points_in_boxes2d", "dg_activate_forward", "dg_activate_backward", "dg_clamp_l1_blocks",
            "dg_clamp_l1_forward", "dg_clamp_l1_backward", "dg_row_prod_forward", "dg_row_prod_backward", "dg_adaptive_capacity", "dg_debug_counters", "dg_adam_update_groups_prox", "dg_train_step", "dg_train_sync",
            "dg_colmap_cameras", "dg_colmap_images", "dg_colmap_points3d", "dg_prune_select", "dg_prune_gather_stats",
+           "dg_adam_update_groups_scaled", "dg_embedding_lookup", "dg_embedding_grad", "dg_embedding_grad_scratch_bytes",
+           "dg_grad_norm", "dg_grad_norm_scratch_bytes", "dg_grad_scale", "dg_clip_grad_norm",
            "dg_last_error", "dg_version", "dg_host_wait_ns", "dg_shutdown")
 
 _lib = None
@@ -294,6 +296,25 @@ def load(path: str | None = None):
             L.dg_ring_destroy.argtypes = [vp]
             L.dg_image_u8_to_chw.restype = C.c_int
             L.dg_image_u8_to_chw.argtypes = [vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp]
+        if hasattr(L, "dg_embedding_lookup"):  # absent in older builds used for A/B runs
+            u32, u64, i64, sz, f64 = C.c_uint32, C.c_uint64, C.c_int64, C.c_size_t, C.c_double
+            L.dg_adam_update_groups_scaled.restype = C.c_int
+            L.dg_adam_update_groups_scaled.argtypes = [C.POINTER(DgAdamGroup), C.POINTER(DgAdamProx), C.c_int, vp, u32,
+                                                       C.c_float, C.c_float, C.POINTER(DgDensifyStats), vp, vp]
+            L.dg_embedding_lookup.restype = C.c_int
+            L.dg_embedding_lookup.argtypes = [vp, C.c_int, u64, u32, i64, i64, vp, C.c_int, u64, C.c_float, vp, vp]
+            L.dg_embedding_grad_scratch_bytes.restype = sz
+            L.dg_embedding_grad_scratch_bytes.argtypes = [u64, u32, u64, C.c_int]
+            L.dg_embedding_grad.restype = C.c_int
+            L.dg_embedding_grad.argtypes = [vp, C.c_int, vp, C.c_int, u64, u64, u32, C.c_float, i64, vp, vp, sz, vp]
+            L.dg_grad_norm_scratch_bytes.restype = sz
+            L.dg_grad_norm_scratch_bytes.argtypes = [C.c_int]
+            L.dg_grad_norm.restype = C.c_int
+            L.dg_grad_norm.argtypes = [C.c_int, vp, vp, vp, C.c_int, f64, vp, vp, vp, sz, vp]
+            L.dg_grad_scale.restype = C.c_int
+            L.dg_grad_scale.argtypes = [C.c_int, vp, vp, vp, vp, vp]
+            L.dg_clip_grad_norm.restype = C.c_int
+            L.dg_clip_grad_norm.argtypes = [C.c_int, vp, vp, vp, C.c_int, f64, vp, vp, sz, vp]
         L.dg_last_error.restype = C.c_char_p
         L.dg_last_error.argtypes = []
         L.dg_version.restype = C.c_int

@@ -22,6 +22,9 @@
 #include "../../include/dogs_hip.h"
 #include "aux_kernels.h"
 #include "blocksplit.h"
+#include "dtypes.h"
+#include "embedding.h"
+#include "gradnorm.h"
 #include "optim.h"
 #include "mask_conv.h"
 #include "export.h"
@@ -1152,11 +1155,17 @@ int dg_adam_update_groups(const dg_adam_group* groups, int n_groups, const uint8
 int dg_adam_update_groups_prox(const dg_adam_group* groups, const dg_adam_prox* prox, int n_groups,
                                const uint8_t* visible, uint32_t N, float b1, float b2, const dg_densify_stats* stats,
                                dg_stream_t stream) {
+    return dg_adam_update_groups_scaled(groups, prox, n_groups, visible, N, b1, b2, stats, nullptr, stream);
+}
+
+int dg_adam_update_groups_scaled(const dg_adam_group* groups, const dg_adam_prox* prox, int n_groups,
+                                 const uint8_t* visible, uint32_t N, float b1, float b2, const dg_densify_stats* stats,
+                                 const double* grad_coef, dg_stream_t stream) {
     if (n_groups < 0 || n_groups > gs::MAX_ADAM_GROUPS) return fail("n_groups must be 0..8%s (got %d)", "", n_groups);
     if (N && !visible) return fail("visible mask required%s%d");
     gs::AdamMultiArgs m;
     memset(&m, 0, sizeof(m));
-    m.visible = visible; m.N = N; m.b1 = b1; m.b2 = b2;
+    m.visible = visible; m.N = N; m.b1 = b1; m.b2 = b2; m.grad_coef = grad_coef;
     int n = 0;
     for (int k = 0; k < n_groups; k++) {
         const dg_adam_group& g = groups[k];
@@ -1180,6 +1189,160 @@ int dg_adam_update_groups_prox(const dg_adam_group* groups, const dg_adam_prox* 
     if (N) gs::launch_adam_multi(m, (hipStream_t)stream);
     HIP_OK(hipGetLastError());
     return 0;
+}
+
+// ---- embedding tables
+
+static int embedding_sizes_ok(const char* what, int dtype, uint64_t V, uint32_t D, uint64_t n) {
+    if (dtype < 0 || dtype > 2) return fail("%s: unknown element type %d", what, dtype);
+    if (V >= (1ull << 31) || n >= (1ull << 31) || D >= (1u << 31)) return fail("%s: V, n and D must be < 2^31%d", what);
+    return 0;
+}
+
+int dg_embedding_lookup(const void* table, int dtype, uint64_t V, uint32_t D, int64_t row_stride, int64_t col_stride,
+                        const void* tokens, int wide, uint64_t n, float scale, void* out, dg_stream_t stream) {
+    API_GUARD();
+    if (embedding_sizes_ok("embedding_lookup", dtype, V, D, n)) return 1;
+    if (n == 0 || D == 0) return 0;
+    if ((!table && V) || !tokens || !out) return fail("embedding_lookup: a tensor is NULL%s%d");
+    gs::LookupArgs a = {table, row_stride, col_stride, tokens, wide != 0, (uint32_t)n, D, V, scale, out};
+    gs::launch_embedding_lookup(a, dtype, (hipStream_t)stream);
+    HIP_OK(hipGetLastError());
+    return 0;
+}
+
+size_t dg_embedding_grad_scratch_bytes(uint64_t V, uint32_t D, uint64_t n, int dtype) {
+    if (V >= (1ull << 31) || n >= (1ull << 31) || dtype < 0 || dtype > 2) return 0;
+    return gs::embedding_grad_scratch_bytes((uint32_t)V, D, (uint32_t)n, dtype);
+}
+
+int dg_embedding_grad(const void* grad, int dtype, const void* tokens, int wide, uint64_t n, uint64_t V, uint32_t D,
+                      float scale, int64_t padding, void* dtable, void* scratch, size_t scratch_bytes,
+                      dg_stream_t stream) {
+    API_GUARD();
+    if (embedding_sizes_ok("embedding_grad", dtype, V, D, n)) return 1;
+    if (V == 0 || D == 0) return 0;
+    if ((n && (!grad || !tokens)) || !dtable || !scratch) return fail("embedding_grad: a tensor is NULL%s%d");
+    if (scratch_bytes < gs::embedding_grad_scratch_bytes((uint32_t)V, D, (uint32_t)n, dtype))
+        return fail("embedding_grad: scratch too small%s%d");
+    gs::LookupGradArgs a = {grad, tokens, wide != 0, (uint32_t)n, D, (uint32_t)V, scale, padding, dtable};
+    gs::launch_embedding_grad(a, dtype, scratch, (hipStream_t)stream);
+    HIP_OK(hipGetLastError());
+    return 0;
+}
+
+// ---- the norm of a set of gradients
+
+// the non-empty tensors, checked
+static int grad_tensors(int n_tensors, const void* const* tensors, const uint64_t* numel, const uint8_t* dtype,
+                        bool distinct, std::vector<gs::GradTable>& tables, uint32_t& blocks) {
+    if (n_tensors < 0 || (n_tensors && (!tensors || !numel || !dtype))) return fail("gradients: bad args%s%d");
+    uint64_t total = 0;
+    for (int k = 0; k < n_tensors; k++) {
+        if (dtype[k] > 2) return fail("gradient %s%d has an unknown element type", "", k);
+        if (!numel[k]) continue;
+        if (numel[k] >= (1ull << 41)) return fail("gradient %s%d is too large", "", k);
+        const uint64_t bytes = numel[k] * gs::elem_bytes(dtype[k]);
+        if (!tensors[k] || (uintptr_t)tensors[k] % gs::elem_bytes(dtype[k]))
+            return fail("gradient %s%d is NULL or not aligned to its elements", "", k);
+        total += bytes;
+        if (total >= (1ull << 43)) return fail("gradients: more than 2^43 bytes%s%d");
+    }
+    const uint32_t chunk = gs::gn_chunk(total);
+    if (distinct) {
+        std::vector<std::pair<uintptr_t, uintptr_t>> r;
+        r.reserve((size_t)n_tensors);
+        for (int k = 0; k < n_tensors; k++)
+            if (numel[k]) r.emplace_back((uintptr_t)tensors[k], (uintptr_t)tensors[k] + numel[k] * gs::elem_bytes(dtype[k]));
+        std::sort(r.begin(), r.end());
+        for (size_t k = 1; k < r.size(); k++)
+            if (r[k].first < r[k - 1].second) return fail("gradients to scale overlap in memory%s%d");
+    }
+    blocks = 0;
+    for (int k = 0; k < n_tensors; k++) {
+        if (!numel[k]) continue;
+        if (tables.empty() || tables.back().count == gs::GN_MAX) {
+            tables.emplace_back();
+            tables.back().count = 0;
+            tables.back().start[0] = 0;
+            tables.back().chunk = chunk;
+        }
+        gs::GradTable& t = tables.back();
+        const uint32_t b = gs::gn_blocks(numel[k], dtype[k], chunk);
+        t.p[t.count] = const_cast<void*>(tensors[k]);
+        t.n[t.count] = numel[k];
+        t.dtype[t.count] = dtype[k];
+        t.start[t.count + 1] = t.start[t.count] + b;
+        t.count++;
+        blocks += b;
+    }
+    return 0;
+}
+
+size_t dg_grad_norm_scratch_bytes(int n_tensors) {
+    return n_tensors < 0 ? 0 : 256 + 8 * ((size_t)gs::GN_MAX_BLOCKS + (size_t)n_tensors);
+}
+
+static int grad_norm_impl(int n_tensors, const void* const* tensors, const uint64_t* numel, const uint8_t* dtype, int ord,
+                          double max_norm, float* norm, double* coef, bool scale, void* scratch, size_t scratch_bytes,
+                          hipStream_t s) {
+    if (!norm || !scratch) return fail("grad_norm: norm and scratch are required%s%d");
+    if (ord < 0 || ord > 2) return fail("grad_norm: ord must be 0, 1 or 2%s (got %d)", "", ord);
+    if ((coef || scale) && !(max_norm >= 0.0)) return fail("grad_norm: max_norm must not be negative%s%d");
+    if (scratch_bytes < dg_grad_norm_scratch_bytes(n_tensors)) return fail("grad_norm: scratch too small%s%d");
+    std::vector<gs::GradTable> tables;
+    uint32_t blocks = 0;
+    if (grad_tensors(n_tensors, tensors, numel, dtype, scale, tables, blocks)) return 1;
+    if (scale) coef = (double*)scratch;
+    double* partial = (double*)((char*)scratch + 256);
+    uint32_t b = 0;
+    for (const gs::GradTable& t : tables) {
+        gs::launch_grad_partials(t, ord, partial + b, s);
+        b += t.start[t.count];
+    }
+    gs::launch_grad_norm_final(partial, blocks, ord, max_norm, norm, coef, s);
+    if (scale)
+        for (const gs::GradTable& t : tables) gs::launch_grad_scale(t, coef, s);
+    HIP_OK(hipGetLastError());
+    return 0;
+}
+
+int dg_grad_norm(int n_tensors, const void* const* tensors, const uint64_t* numel, const uint8_t* dtype, int ord,
+                 double max_norm, float* norm, double* coef, void* scratch, size_t scratch_bytes, dg_stream_t stream) {
+    API_GUARD();
+    try {
+        return grad_norm_impl(n_tensors, tensors, numel, dtype, ord, max_norm, norm, coef, false, scratch, scratch_bytes,
+                              (hipStream_t)stream);
+    } catch (const std::exception& e) {
+        return fail("grad_norm: %s%d", e.what());
+    }
+}
+
+int dg_grad_scale(int n_tensors, void* const* tensors, const uint64_t* numel, const uint8_t* dtype, const double* coef,
+                  dg_stream_t stream) {
+    API_GUARD();
+    try {
+        if (!coef) return fail("grad_scale: coef is required%s%d");
+        std::vector<gs::GradTable> tables;
+        uint32_t blocks = 0;
+        if (grad_tensors(n_tensors, tensors, numel, dtype, true, tables, blocks)) return 1;
+        for (const gs::GradTable& t : tables) gs::launch_grad_scale(t, coef, (hipStream_t)stream);
+        HIP_OK(hipGetLastError());
+        return 0;
+    } catch (const std::exception& e) {
+        return fail("grad_scale: %s%d", e.what());
+    }
+}
+
+int dg_clip_grad_norm(int n_tensors, void* const* tensors, const uint64_t* numel, const uint8_t* dtype, int ord,
+                      double max_norm, float* norm, void* scratch, size_t scratch_bytes, dg_stream_t stream) {
+    API_GUARD();
+    try {
+        return grad_norm_impl(n_tensors, tensors, numel, dtype, ord, max_norm, norm, nullptr, true, scratch, scratch_bytes,
+                              (hipStream_t)stream);
+    } catch (const std::exception& e) {
+        return fail("clip_grad_norm: %s%d", e.what());
+    }
 }
 
 int dg_train_step(const dg_train_step_args* a, dg_alloc_fn alloc, void* user, dg_stream_t stream) {

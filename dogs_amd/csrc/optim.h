@@ -63,6 +63,7 @@ struct AdamMultiArgs {
     // instead of visible / vis_radii / hot (the next step's forward overwrites those while the launch may still run)
     uint8_t* status_out;
     const uint8_t* status;
+    const double* grad_coef;  // optional (device): every gradient times *grad_coef before the proximal term
     uint32_t grid_cap;   // optional: at most this many blocks, striding over the work (0: one block per work block)
     uint32_t nblocks;    // set by launch_adam_multi
 };

@@ -192,6 +192,11 @@ __device__ __forceinline__ void adam_block(const AdamMultiArgs& a, const uint32_
         } else if (g.gmode == 3) {
             gr[c] = normalize_bwd(p[c], gr[c]);  // M = 4: the chunk is the row
         }
+        if (a.grad_coef) {  // the clipping coefficient of the step's gradient norm
+            const double c1 = *a.grad_coef;
+            gr[c].x = (float)(gr[c].x * c1); gr[c].y = (float)(gr[c].y * c1);
+            gr[c].z = (float)(gr[c].z * c1); gr[c].w = (float)(gr[c].w * c1);
+        }
         if (g.u) {  // the ADMM proximal gradient joins the loss gradient before the moments see it
             float4 u, z;
             if (full[c]) {

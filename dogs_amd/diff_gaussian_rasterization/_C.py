@@ -395,13 +395,14 @@ def _group_array(chunk, N):
     return arr
 
 
-def adam_update_groups(groups, visible, N, b1=0.9, b2=0.999, stats=None, prox=None):
+def adam_update_groups(groups, visible, N, b1=0.9, b2=0.999, stats=None, prox=None, grad_coef=None):
     """SparseGaussianAdam over several groups in one launch (dg_adam_update_groups; each group as adamUpdate).
     groups: iterable of (param, grad, exp_avg, exp_avg_sq, lr, eps); stats (optional): dict with radii [N] int32,
     dmeans2D [N,>=2] (screen-space-point gradient), max_radii2D [N], grad_accum [N(,1)], denom [N(,1)] -- the view's
     densification statistics (gaussian_trainer.py:433-438), updated in the same launch.  prox (optional): one entry
     per group, None or (u, z, coef) -- the ADMM penalty 0.5 rho mse(x + u, z) of a block trainer as its gradient
-    coef ((x + u) - z), coef = rho / numel(x), added for the rows Adam updates (dg_adam_update_groups_prox)."""
+    coef ((x + u) - z), coef = rho / numel(x), added for the rows Adam updates (dg_adam_update_groups_prox).  grad_coef
+    (optional): a 0-d float64 on the device that every gradient is multiplied by as it is read, in one rounding."""
     groups = list(groups)
     prox = list(prox) if prox is not None else None
     if prox is not None and len(prox) != len(groups):
@@ -451,7 +452,10 @@ def adam_update_groups(groups, visible, N, b1=0.9, b2=0.999, stats=None, prox=No
                         keep += [u, z]
                         parr[i] = _lib.DgAdamProx(u.data_ptr(), z.data_ptr(), float(coef))
             st_p = C.byref(st) if (st is not None and c0 == 0) else None
-            if parr is not None:
+            if grad_coef is not None:
+                _lib.check(L.dg_adam_update_groups_scaled(arr, parr, len(chunk), vis.data_ptr(), int(N), float(b1),
+                                                          float(b2), st_p, grad_coef.data_ptr(), _lib.stream_of(dev)))
+            elif parr is not None:
                 _lib.check(L.dg_adam_update_groups_prox(arr, parr, len(chunk), vis.data_ptr(), int(N), float(b1),
                                                         float(b2), st_p, _lib.stream_of(dev)))
             else:

@@ -207,9 +207,16 @@ class SparseGaussianAdam(torch.optim.Adam):
         super().__init__(params=params, lr=lr, eps=eps)
 
     @torch.no_grad()
-    def step(self, visibility, N, stats=None, prox=None):
+    def step(self, visibility, N, stats=None, prox=None, max_norm=None):
         """prox (optional): {group name: (u, z, coef)} -- an ADMM block trainer's penalty gradient folded into the
-        same launch (_C.adam_update_groups)."""
+        same launch (_C.adam_update_groups).
+
+        max_norm (optional): clip by the norm of all groups' gradients, every row's, as clip_grad_norm_ before the step
+        would; the update multiplies the gradients by min(1, max_norm / (norm + 1e-6)) as it reads them, and they stay
+        as they are.  Returns the norm then, a 0-d float32 on the device (None without max_norm).  The penalty of prox
+        is no part of the gradients here: the two together are refused."""
+        if max_norm is not None and prox is not None:
+            raise RuntimeError("step: max_norm does not see the penalty of prox: give one of the two")
         groups = []
         proxes = []
         for group in self.param_groups:
@@ -227,6 +234,25 @@ class SparseGaussianAdam(torch.optim.Adam):
             grad = param.grad if param.grad.is_contiguous() else param.grad.contiguous()
             groups.append((param, grad, state["exp_avg"], state["exp_avg_sq"], lr, eps))
             proxes.append(None if prox is None else prox.get(group.get("name")))
+        norm = coef = None
+        if max_norm is not None:
+            norm, coef = _clip(groups, visibility, N, max_norm)
         if groups or stats is not None:
             _C.adam_update_groups(groups, visibility, N, 0.9, 0.999, stats,
-                                  prox=proxes if prox is not None else None)
+                                  prox=proxes if prox is not None else None, grad_coef=coef)
+        return norm
+
+
+def _clip(groups, visibility, N, max_norm):
+    """(norm, coefficient) of a step's gradients."""
+    from ..gradclip import clip_coefficient
+    if visibility.numel() != N:
+        raise RuntimeError(f"step: visibility has {visibility.numel()} entries for {N} rows")
+    for param, grad, m, v, _, _ in groups:
+        _C._check_group(param, grad, m, v)
+        if param.device != visibility.device or any(t.device != param.device or t.numel() != param.numel()
+                                                    for t in (grad, m, v)) or (param.numel() % N if N else param.numel()):
+            raise RuntimeError(f"step: a group's tensors are not {N} rows each on {visibility.device}")
+    if not groups:
+        return torch.zeros((), device=visibility.device), None
+    return clip_coefficient([g[1] for g in groups], max_norm)

@@ -1,0 +1,146 @@
+"""The norm of a set of gradients, and clipping by it, through dg_grad_norm / dg_clip_grad_norm (gradnorm.hip): the
+steps of torch.nn.utils.clip_grad_norm_ in a few launches whatever the number of tensors, with 64-bit sums in a fixed order.
+SparseGaussianAdam.step(max_norm=...) clips without rewriting the gradients."""
+from __future__ import annotations
+
+import math
+from array import array
+from typing import Iterable
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # dogs_hip.h DG_F32, DG_F16, DG_BF16
+_ORDERS = {2.0: 2, 1.0: 1, math.inf: 0}
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether t's elements fill one stretch of memory, in any order of its dimensions (channels last, transposed)."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+class _Table:
+    """The tensors of a call as the library takes them; keeps what it points at."""
+
+    def __init__(self, tensors: list, name: str, in_place: bool):
+        dev = tensors[0].device
+        ptrs, sizes, types = array("Q"), array("Q"), bytearray()
+        self.keep, self.copies = [], []
+        for t in tensors:
+            code = _DTYPES.get(t.dtype)
+            if code is None or not t.is_cuda or t.device != dev or t.layout != torch.strided:
+                raise RuntimeError(f"{name}: gradients must be dense float32, float16 or bfloat16 tensors on one HIP "
+                                   f"device, got {t.dtype} {t.layout} on {t.device}")
+            if not t.is_contiguous() and not _dense(t):
+                c = t.contiguous()
+                if in_place:
+                    if any(st == 0 and sz > 1 for st, sz in zip(t.stride(), t.shape)):
+                        raise RuntimeError(f"{name}: a gradient's elements share memory: it cannot be scaled in place")
+                    self.copies.append((t, c))
+                self.keep.append(c)
+                t = c
+            ptrs.append(t.data_ptr())
+            sizes.append(t.numel())
+            types.append(code)
+        self.device, self.n = dev, len(ptrs)
+        self.ptrs, self.sizes, self.types = ptrs, sizes, array("B", types)
+
+    @property
+    def args(self) -> tuple:
+        return (self.n, self.ptrs.buffer_info()[0], self.sizes.buffer_info()[0], self.types.buffer_info()[0])
+
+    def write_back(self) -> None:
+        for t, c in self.copies:
+            t.copy_(c)
+
+
+def _order(name: str, norm_type) -> int:
+    order = _ORDERS.get(float(norm_type))
+    if order is None:
+        raise RuntimeError(f"{name}: norm_type must be 1, 2 or inf, got {norm_type}")
+    return order
+
+
+def _max_norm(name: str, max_norm) -> float:
+    m = float(max_norm)
+    if not m >= 0.0:
+        raise RuntimeError(f"{name}: max_norm must not be negative, got {max_norm}")
+    return m
+
+
+def _scratch(L, t: _Table) -> tuple:
+    nbytes = L.dg_grad_norm_scratch_bytes(t.n)
+    return torch.empty(nbytes, dtype=torch.uint8, device=t.device), nbytes
+
+
+def grad_norm(tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
+    """The norm of all elements of the tensors together (norm_type 2, 1 or inf), a 0-d float32 on their device.  float32,
+    float16 and bfloat16 may be mixed; no tensors: 0."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    order = _order("grad_norm", norm_type)
+    if not tensors:
+        return torch.tensor(0.0)
+    t = _Table(tensors, "grad_norm", in_place=False)
+    L = _lib.load()
+    norm = torch.empty((), dtype=torch.float32, device=t.device)
+    scratch, nbytes = _scratch(L, t)
+    with _lib.device_ctx(t.device):
+        _lib.check(L.dg_grad_norm(*t.args, order, 0.0, norm.data_ptr(), None, scratch.data_ptr(), nbytes,
+                                  _lib.stream_of(t.device)))
+    return norm
+
+
+def clip_coefficient(tensors: list, max_norm: float) -> tuple:
+    """(norm, coefficient) of the tensors' 2-norm: the norm a 0-d float32, the coefficient min(1, max_norm / (norm + 1e-6)) a
+    0-d float64, on the device.  For a step that scales the gradients as it reads them."""
+    max_norm = _max_norm("clip_coefficient", max_norm)
+    t = _Table(tensors, "clip_coefficient", in_place=False)
+    L = _lib.load()
+    norm = torch.empty((), dtype=torch.float32, device=t.device)
+    coef = torch.empty((), dtype=torch.float64, device=t.device)
+    scratch, nbytes = _scratch(L, t)
+    with _lib.device_ctx(t.device):
+        _lib.check(L.dg_grad_norm(*t.args, 2, max_norm, norm.data_ptr(), coef.data_ptr(), scratch.data_ptr(), nbytes,
+                                  _lib.stream_of(t.device)))
+    return norm, coef
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """torch.nn.utils.clip_grad_norm_: scales the parameters' gradients in place by min(1, max_norm / (norm + 1e-6)) of
+    the norm of them all (norm_type 2, 1 or inf) and returns that norm, a 0-d float32 on their device.  Gradients within
+    max_norm are not written at all.  Parameters without a gradient are left out, and one that is given twice
+    counts once; gradients that share memory are refused.  A norm that is NaN makes every gradient NaN, an infinite one
+    makes them 0 (NaN where they were infinite), unless error_if_nonfinite, which reads the norm back and raises."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    order, max_norm = _order("clip_grad_norm_", norm_type), _max_norm("clip_grad_norm_", max_norm)
+    grads = [p.grad for p in dict.fromkeys(parameters) if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    t = _Table(grads, "clip_grad_norm_", in_place=True)
+    L = _lib.load()
+    norm = torch.empty((), dtype=torch.float32, device=t.device)
+    scratch, nbytes = _scratch(L, t)
+    with _lib.device_ctx(t.device):
+        stream = _lib.stream_of(t.device)
+        if error_if_nonfinite:
+            coef = torch.empty((), dtype=torch.float64, device=t.device)
+            _lib.check(L.dg_grad_norm(*t.args, order, max_norm, norm.data_ptr(), coef.data_ptr(), scratch.data_ptr(),
+                                      nbytes, stream))
+            if not math.isfinite(float(norm)):
+                raise RuntimeError(f"clip_grad_norm_: the norm of the gradients is {float(norm)}")
+            _lib.check(L.dg_grad_scale(*t.args, coef.data_ptr(), stream))
+        else:
+            _lib.check(L.dg_clip_grad_norm(*t.args, order, max_norm, norm.data_ptr(), scratch.data_ptr(), nbytes, stream))
+        t.write_back()
+    torch.autograd.graph.increment_version(grads)
+    return norm

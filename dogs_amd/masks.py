@@ -141,19 +141,44 @@ class AppearanceEmbedding(nn.Module):
 
     def forward(self, image: torch.Tensor, index: int, image_size: tuple) -> torch.Tensor:
         """image: [3, h, w] (the 32x-downsampled target); index: the view's row of the embedding table;
-        image_size: (H, W) of the render.  Returns the [3, H, W] mask."""
+        image_size: (H, W) of the render.  Returns the [3, H, W] mask.
+
+        A batch of B views of one size: image [B, 3, h, w] and index an int tensor [B] (on the device or the host);
+        returns [B, 3, H, W].  The codes are then one embedding_lookup, and the table's gradient its sorted sums: a view
+        that is in the batch twice adds both."""
+        if image.dim() == 4:
+            return self._forward_batch(image, index, image_size)
         _, h, w = image.shape
         code = self.appearance_embedding[index]
         x = torch.cat([image, code[:, None, None].expand(code.shape[0], h, w)], dim=0)
         x = self.fusion(x)
         for st in self.upsample:   # (PixelShuffle, Conv3x3, ReLU): shuffle and ReLU folded into the convolution's kernels
             x = st[1](x, relu=True, shuffle=True)
+        return self._head(x, image_size)
+
+    def _head(self, x: torch.Tensor, image_size: tuple) -> torch.Tensor:
         H, W = int(image_size[0]), int(image_size[1])
         if x.is_cuda and x.dim() == 3 and H <= 4 * x.shape[1] and W <= 4 * x.shape[2]:
             c1, c2 = self.out_conv[0], self.out_conv[2]
             return _MaskHead.apply(x, c1.weight, c1.bias, c2.weight, c2.bias, (H, W))
         x = resize_bilinear(x, (H, W))
         return self.out_conv(x)
+
+    def _forward_batch(self, images: torch.Tensor, index: torch.Tensor, image_size: tuple) -> torch.Tensor:
+        B, _, h, w = images.shape
+        if not isinstance(index, torch.Tensor) or tuple(index.shape) != (B,):
+            raise ValueError(f"AppearanceEmbedding: a batch of {B} images takes an int tensor of {B} view indices")
+        table = self.appearance_embedding
+        if table.is_cuda:
+            from .embedding import embedding_lookup
+            codes = embedding_lookup(table, index)
+        else:
+            codes = F.embedding(index, table)
+        x = torch.cat([images, codes[:, :, None, None].expand(B, codes.shape[1], h, w)], dim=1)
+        x = self.fusion(x)
+        for st in self.upsample:
+            x = st[1](x, relu=True, shuffle=True)
+        return torch.stack([self._head(v, image_size) for v in x])
 
 
 class _MaskHead(torch.autograd.Function):
@@ -292,8 +317,9 @@ class MaskedStep:
     on the target and the view's embedding), hands dg_train_step the mask and a dL/dmask buffer, then runs the
     network's backward and its Adam step (gaussian_trainer.py:482-484).  `small` caches the 32x-downsampled targets."""
 
-    def __init__(self, net: AppearanceEmbedding, optimizer: torch.optim.Optimizer):
-        self.net, self.opt = net, optimizer
+    def __init__(self, net: AppearanceEmbedding, optimizer: torch.optim.Optimizer, max_grad_norm: float = 0.0):
+        """max_grad_norm > 0: the network's gradients are clipped to this norm before its step."""
+        self.net, self.opt, self.max_grad_norm = net, optimizer, float(max_grad_norm)
         self.small: dict = {}
         self.mask = None
         self.dmask: dict = {}
@@ -317,8 +343,14 @@ class MaskedStep:
         self._m = m
         return m, buf
 
+    def clip(self) -> None:
+        if self.max_grad_norm > 0.0:
+            from .gradclip import clip_grad_norm_
+            clip_grad_norm_(self.net.parameters(), self.max_grad_norm)
+
     def backward_and_step(self, dmask: torch.Tensor) -> None:
         self.mask.backward(dmask)
+        self.clip()
         self.opt.step()
         self.opt.zero_grad(set_to_none=True)
         self.mask = self._m = None

@@ -32,6 +32,11 @@ Options of the reference configs (GSTrainConfig.from_reference reads them from t
         302-307, 478-480); such iterations take the autograd route (the exposure mixes the render's channels before the
         clamp, which the native step's fused loss does not model).
     geometry.coarse-to-fine: training_resolution (:309-319); downsampled iterations take the autograd route.
+
+Clipping (no reference key): max_grad_norm > 0 clips the six tensors' gradients by their common norm inside
+SparseGaussianAdam.step; every iteration then takes the autograd route, because the native step folds the activations'
+backward into its update and never holds the gradients that the norm is of.  mask_max_grad_norm > 0 clips the appearance
+embedding's with clip_grad_norm_, on both routes.  last_grad_norm is the last iteration's norm before clipping.
 """
 from __future__ import annotations
 
@@ -91,6 +96,8 @@ class GSTrainConfig:
     exposure_lr_delay_mult: float = 0.0
     exposure_max_iterations: int | None = None   # ${trainer.max_iterations}
     coarse_to_fine: bool = False        # geometry.coarse-to-fine
+    max_grad_norm: float = 0.0          # > 0: clip the Gaussians' gradients to this norm (no reference key)
+    mask_max_grad_norm: float = 0.0     # > 0: and the appearance embedding's to this one
 
     @classmethod
     def from_reference(cls, config) -> "GSTrainConfig":
@@ -233,7 +240,7 @@ class GaussianSplatTrainer:
             # iteration); the same optimizer in both routes and in every ADMM rank
             self.mask_optimizer = torch.optim.Adam(self.mask.parameters(), lr=c.mask_lr,
                                                    fused=self.device.type == "cuda")
-            self._masked = MaskedStep(self.mask, self.mask_optimizer)
+            self._masked = MaskedStep(self.mask, self.mask_optimizer, c.mask_max_grad_norm)
         # the trained exposure and its Adam + schedule (:246-257); the model holds one [3,4] per training image
         self.exposure_optimizer = self.exposure_scheduler = None
         if c.use_trained_exposure:
@@ -247,6 +254,7 @@ class GaussianSplatTrainer:
         self._nts = None
         self._nts_stats = None
         self.last_loss = None
+        self.last_grad_norm = None
         self._scaled_views: dict = {}
 
     # ---- helpers
@@ -357,7 +365,7 @@ class GaussianSplatTrainer:
         k = self._next_view()
         ev = self._events()
         res = self.training_resolution()
-        if self.native and not ev and res == 1 and self.exposure_optimizer is None:
+        if self.native and not ev and res == 1 and self.exposure_optimizer is None and c.max_grad_norm <= 0.0:
             nts = self._native_step()
             mask = dmask = None
             if self._masked is not None:
@@ -424,12 +432,16 @@ class GaussianSplatTrainer:
                 i = list(c.prune_iterations).index(self.iteration)
                 m.prune_gaussians_with_opt((c.prune_decay ** i) * c.prune_percent, v, self.optimizer)
                 replaced = True
-        self.optimizer.step(radii > 0, radii.shape[0])
+        if c.max_grad_norm > 0.0:
+            self.last_grad_norm = self.optimizer.step(radii > 0, radii.shape[0], max_norm=c.max_grad_norm)
+        else:
+            self.optimizer.step(radii > 0, radii.shape[0])
         self.optimizer.zero_grad(set_to_none=True)
         if self.exposure_optimizer is not None:    # :478-480
             self.exposure_optimizer.step()
             self.exposure_optimizer.zero_grad(set_to_none=True)
         if self.mask_optimizer is not None:        # :482-484
+            self._masked.clip()
             self.mask_optimizer.step()
             self.mask_optimizer.zero_grad(set_to_none=True)
         if replaced:

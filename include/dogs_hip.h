@@ -228,6 +228,43 @@ typedef struct {
 int dg_adam_update_groups_prox(const dg_adam_group* groups, const dg_adam_prox* prox, int n_groups,
                                const uint8_t* visible, uint32_t N, float b1, float b2, const dg_densify_stats* stats,
                                dg_stream_t stream);
+/* dg_adam_update_groups_prox with every gradient (the penalty's apart) times *grad_coef first, a device scalar such as
+ * dg_grad_norm's clipping coefficient, in one rounding: the clipped step without a pass that rewrites the gradients.  NULL: as given. */
+int dg_adam_update_groups_scaled(const dg_adam_group* groups, const dg_adam_prox* prox, int n_groups,
+                                 const uint8_t* visible, uint32_t N, float b1, float b2, const dg_densify_stats* stats,
+                                 const double* grad_coef, dg_stream_t stream);
+
+/* ---- embedding tables, and the norm of a set of gradients ---- */
+enum { DG_F32 = 0, DG_F16 = 1, DG_BF16 = 2 };   /* element types */
+
+/* out [n][D] = scale * table[tokens[i]], in table's type (products in 32 bits, rounded once).  table: V rows of D elements,
+ * element (v, c) at v * row_stride + c * col_stride (in elements); tokens: n of 32 or (wide) 64 bits.  A token outside
+ * [0, V) reads nothing and its row of out is NaN.  n, V < 2^31. */
+int dg_embedding_lookup(const void* table, int dtype, uint64_t V, uint32_t D, int64_t row_stride, int64_t col_stride,
+                        const void* tokens, int wide, uint64_t n, float scale, void* out, dg_stream_t stream);
+/* Its gradient for the table: dtable [V][D] (every element is written) = scale * sum of the rows i of grad [n][D] with
+ * tokens[i] == v, for every v != padding (-1: none); sums in 32 bits in an order that only the tokens set, without
+ * atomics.  Tokens outside [0, V) add nothing.  scratch of dg_embedding_grad_scratch_bytes(V, D, n, dtype) bytes. */
+size_t dg_embedding_grad_scratch_bytes(uint64_t V, uint32_t D, uint64_t n, int dtype);
+int dg_embedding_grad(const void* grad, int dtype, const void* tokens, int wide, uint64_t n, uint64_t V, uint32_t D,
+                      float scale, int64_t padding, void* dtable, void* scratch, size_t scratch_bytes,
+                      dg_stream_t stream);
+
+/* *norm = the norm of all elements of n_tensors tensors (contiguous, numel[k] elements of type dtype[k]): ord 2 the root of
+ * the sum of squares, 1 the sum of |x|, 0 the largest |x|; sums in 64 bits, in a fixed order.  coef (may be NULL): *coef =
+ * min(1, max_norm / (norm + 1e-6)), in 64 bits: next to a norm near fp32's limit it is below fp32's normal range.  The pointer arrays are read during the call only.  scratch of
+ * dg_grad_norm_scratch_bytes(n_tensors) bytes. */
+size_t dg_grad_norm_scratch_bytes(int n_tensors);
+int dg_grad_norm(int n_tensors, const void* const* tensors, const uint64_t* numel, const uint8_t* dtype, int ord,
+                 double max_norm, float* norm, double* coef, void* scratch, size_t scratch_bytes, dg_stream_t stream);
+/* Every element of the tensors times *coef (a device scalar), in place; with *coef == 1 nothing is written.  The tensors
+ * must not overlap (an error). */
+int dg_grad_scale(int n_tensors, void* const* tensors, const uint64_t* numel, const uint8_t* dtype, const double* coef,
+                  dg_stream_t stream);
+/* Both: *norm as dg_grad_norm and, when it exceeds max_norm, the tensors scaled down to it. */
+int dg_clip_grad_norm(int n_tensors, void* const* tensors, const uint64_t* numel, const uint8_t* dtype, int ord,
+                      double max_norm, float* norm, void* scratch, size_t scratch_bytes, dg_stream_t stream);
+
 /* ---- the native training step of a block trainer (dogs_amd.admm_trainer.BlockTrainer's fast path) ----
  * One GaussianSplatTrainer.train_iteration after densify_end_iter (gaussian_trainer.py:324-476) with the ADMM
  * penalty of SlaveGaussianSplatTrainer.add_admm_penalties (slave_gaussian_trainer.py:161-202), as one call:

@@ -1,0 +1,345 @@
+"""grad_norm, clip_grad_norm_ and SparseGaussianAdam.step(max_norm=...) against the formulas in 64 bits.
+
+Tolerances, from the arithmetic (u = 2^-24; h = half a step of the gradient's type): the squares and sums are 64-bit, so the
+norm is off by its one rounding to fp32, u, and the test's own 64-bit sums by far less: 2 u.  A clipped gradient: the
+coefficient and the product in 64 bits, their rounding to fp32 u, the result h: |g c| (h + 3 u), and half of fp16's smallest subnormal."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TINY = {torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134}
+SETS = {
+    "one": [((1,), torch.float32)],
+    "odd": [((3, 5, 7), torch.float32), ((1,), torch.bfloat16), ((12345,), torch.float16), ((0, 4), torch.float32),
+            ((4097, 3), torch.bfloat16)],
+    "scene": [((30011, w), torch.float32) for w in (3, 3, 45, 1, 3, 4)],
+    "many": [((k % 97 + 1, k % 5 + 1), (torch.float32, torch.float16, torch.bfloat16)[k % 3]) for k in range(300)],
+    "exactly a table": [((17,), torch.float32) for _ in range(128)],
+    "a table and one": [((17,), torch.float32) for _ in range(129)],
+    "large": [((5000, 4099), torch.bfloat16), ((70001,), torch.float32), ((4096, 4096), torch.float32)],
+}
+
+
+def _grads(dev, name, seed=0, std=1.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return [(torch.randn(s, generator=g, device=dev) * std).to(t) for s, t in SETS[name]]
+
+
+def _params(grads):
+    ps = []
+    for g in grads:
+        p = torch.nn.Parameter(torch.empty_like(g))
+        p.grad = g
+        ps.append(p)
+    return ps
+
+
+def _norm(grads, order=2.0):
+    flat = [g.double().abs() for g in grads if g.numel()]
+    if order == 2.0:
+        return math.sqrt(math.fsum(float((g * g).sum()) for g in flat))
+    return math.fsum(float(g.sum()) for g in flat) if order == 1.0 else max(float(g.max()) for g in flat)
+
+
+@pytest.mark.parametrize("order", [2.0, 1.0, math.inf])
+@pytest.mark.parametrize("name", list(SETS))
+def test_norm(hip_device, name, order):
+    from dogs_amd.gradclip import grad_norm
+    grads = _grads(hip_device, name)
+    got = grad_norm(grads, order)
+    assert got.shape == () and got.dtype == torch.float32 and got.device == hip_device
+    want = _norm(grads, order)
+    assert abs(float(got) - want) <= 2 * U * want
+    assert torch.equal(got, grad_norm(grads, order))
+    assert torch.equal(got, grad_norm(iter(grads), norm_type=order))
+
+
+@pytest.mark.parametrize("order", [2.0, 1.0, math.inf])
+@pytest.mark.parametrize("part", [0.25, 0.999, 1.5, 0.0])
+@pytest.mark.parametrize("name", list(SETS))
+def test_clip(hip_device, name, part, order):
+    from dogs_amd.gradclip import clip_grad_norm_
+    grads = _grads(hip_device, name, seed=1)
+    old = [g.clone() for g in grads]
+    n = _norm(old, order)
+    limit = part * n
+    got = clip_grad_norm_(_params(grads), limit, norm_type=order)
+    assert abs(float(got) - n) <= 2 * U * n
+    c = min(1.0, limit / (n + 1e-6))
+    for g, o in zip(grads, old):
+        if c == 1.0:
+            assert torch.equal(g, o)
+            continue
+        want = o.double() * c
+        tol = want.abs() * (torch.finfo(o.dtype).eps / 2 + 3 * U) + TINY[o.dtype]
+        assert bool(((g.double() - want).abs() <= tol).all())
+
+
+def test_agrees_with_torch(hip_device):
+    from dogs_amd.gradclip import clip_grad_norm_
+    a, b = (_params(_grads(hip_device, "scene", seed=2)) for _ in range(2))
+    a.append(torch.nn.Parameter(torch.zeros(3, device=hip_device)))    # no gradient
+    n, m = clip_grad_norm_(a, 0.7), torch.nn.utils.clip_grad_norm_(b, 0.7)
+    assert abs(float(n) - float(m)) <= 1e-5 * float(m)                 # its sums are 32-bit
+    for p, q in zip(a, b):
+        assert torch.allclose(p.grad, q.grad, rtol=2e-5, atol=0.0)
+
+
+def test_no_gradient_is_too_large_or_small(hip_device):
+    """Squares past fp32's range in both directions; the norm itself past it; subnormal gradients."""
+    from dogs_amd.gradclip import clip_grad_norm_, grad_norm
+    for x in (1e30, 1e-30, 3e38, 2.0 ** -140):
+        g = torch.full((1000,), x, device=hip_device)
+        want = float(g[0].double()) * math.sqrt(1000)
+        if want > torch.finfo(torch.float32).max:
+            assert math.isinf(float(grad_norm([g])))
+        else:
+            assert abs(float(grad_norm([g])) - want) <= 2 * U * want + 2.0 ** -150
+        p = _params([g])
+        clip_grad_norm_(p, 1.0)
+        c = min(1.0, 1.0 / (want + 1e-6))
+        assert abs(float(g[7]) - x * c) <= 4 * U * x * c + 2.0 ** -149
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("order", [2.0, 1.0, math.inf])
+def test_nonfinite(hip_device, bad, order):
+    from dogs_amd.gradclip import clip_grad_norm_, grad_norm
+    grads = _grads(hip_device, "odd", seed=3)
+    grads[2][777] = bad
+    norm = float(grad_norm(grads, order))
+    assert math.isnan(norm) if math.isnan(bad) else norm == math.inf
+    keep = [g.clone() for g in grads]
+    with pytest.raises(RuntimeError):
+        clip_grad_norm_(_params(grads), 1.0, norm_type=order, error_if_nonfinite=True)
+    assert all(torch.equal(a[a == a], b[b == b]) for a, b in zip(grads, keep))     # not touched
+    clip_grad_norm_(_params(grads), 1.0, norm_type=order)
+    for k, g in enumerate(grads):
+        if math.isnan(bad):
+            assert bool(g.isnan().all())
+        else:
+            zero = g.clone()
+            if k == 2:
+                assert math.isnan(float(g[777]))
+                zero[777] = 0
+            assert not zero.any()
+
+
+def test_strides_and_views(hip_device):
+    """Channels last, transposed, slices of one buffer at unaligned offsets, and gapped slices."""
+    from dogs_amd.gradclip import clip_grad_norm_, grad_norm
+    g = torch.Generator(device=hip_device).manual_seed(4)
+    flat = torch.randn(5000, generator=g, device=hip_device)
+    half = torch.randn((60, 50), generator=g, device=hip_device).to(torch.bfloat16)
+    grads = [torch.randn((4, 6, 5, 3), generator=g, device=hip_device).to(memory_format=torch.channels_last),
+             torch.randn((40, 30), generator=g, device=hip_device).t(), flat[1:1002], flat[1002:1003], flat[2001:4000],
+             half[3:50, 7:40], half.t()[41:, ::2]]
+    want = _norm(grads)
+    assert abs(float(grad_norm(grads)) - want) <= 2 * U * want
+    old = [x.clone() for x in grads]
+    rest = flat[1003:2001].clone(), flat[4000:].clone(), half[:3].clone()
+    ps = []
+    for x in grads:
+        p = torch.nn.Parameter(torch.empty(x.shape, dtype=x.dtype, device=hip_device))
+        p.grad = x
+        ps.append(p)
+    clip_grad_norm_(ps, want / 2)
+    for x, o in zip(grads, old):
+        w = o.double() * (want / 2 / (want + 1e-6))
+        assert bool(((x.double() - w).abs() <= w.abs() * (torch.finfo(o.dtype).eps / 2 + 3 * U)).all())
+    assert torch.equal(flat[1003:2001], rest[0]) and torch.equal(flat[4000:], rest[1])
+    assert torch.equal(half[:3, :40], rest[2][:, :40])
+    wide = torch.randn(3, generator=g, device=hip_device)[:, None].expand(3, 50)     # a broadcast gradient: read, not scaled
+    assert abs(float(grad_norm(wide)) - _norm([wide])) <= 2 * U * _norm([wide])
+    p = torch.nn.Parameter(torch.zeros((3, 50), device=hip_device))
+    p.grad = wide
+    with pytest.raises(RuntimeError):
+        clip_grad_norm_(p, 1.0)
+
+
+def test_shared_gradients(hip_device):
+    """A parameter given twice counts once; two parameters whose gradients overlap are refused, with nothing written."""
+    from dogs_amd.gradclip import clip_grad_norm_
+    g = torch.full((100,), 3.0, device=hip_device)
+    p, = _params([g])
+    assert float(clip_grad_norm_([p, p], 15.0)) == 30.0
+    assert abs(float(g[5]) - 1.5) <= 1e-6
+    flat = torch.full((100,), 3.0, device=hip_device)
+    a, b = torch.nn.Parameter(torch.zeros(60, device=hip_device)), torch.nn.Parameter(torch.zeros(60, device=hip_device))
+    a.grad, b.grad = flat[:60], flat[40:]
+    with pytest.raises(RuntimeError, match="overlap"):
+        clip_grad_norm_([a, b], 1.0)
+    assert bool((flat == 3.0).all())
+
+
+def test_past_32_bit_sizes(hip_device):
+    from dogs_amd.gradclip import clip_grad_norm_, grad_norm
+    n = 2 ** 32 + 12345
+    g = torch.full((n,), 0.5, dtype=torch.bfloat16, device=hip_device)
+    want = 0.5 * math.sqrt(n)
+    assert abs(float(grad_norm(g)) - want) <= 2 * U * want
+    p, = _params([g])
+    clip_grad_norm_(p, want / 2)
+    assert float(g[0]) == float(g[-1]) == 0.25 and bool((g[2 ** 31 - 5:2 ** 31 + 5] == 0.25).all())
+    assert bool((g[-20000:] == 0.25).all())
+
+
+def test_empty_and_refusals(hip_device):
+    from dogs_amd.gradclip import clip_grad_norm_, grad_norm
+    assert float(grad_norm([])) == 0.0 and float(clip_grad_norm_([], 1.0)) == 0.0
+    assert float(grad_norm(torch.empty(0, device=hip_device))) == 0.0
+    p = torch.nn.Parameter(torch.zeros(3, device=hip_device))
+    assert float(clip_grad_norm_(p, 1.0)) == 0.0
+    p.grad = torch.ones(3, device=hip_device)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(RuntimeError):
+            clip_grad_norm_(p, bad)
+    for order in (3.0, 0.0, -1.0, 0.5, -math.inf):
+        with pytest.raises(RuntimeError):
+            clip_grad_norm_(p, 1.0, norm_type=order)
+    for t in (torch.ones(3), torch.ones(3, device=hip_device).double(), torch.ones(3, device=hip_device).int(),
+              torch.eye(3, device=hip_device).to_sparse()):
+        with pytest.raises(RuntimeError):
+            grad_norm([torch.ones(3, device=hip_device), t])
+    assert torch.equal(p.grad, torch.ones(3, device=hip_device))
+
+
+def test_in_place_change_is_seen_by_autograd(hip_device):
+    from dogs_amd.gradclip import clip_grad_norm_
+    p, = _params([torch.ones(8, device=hip_device)])
+    x = torch.ones(8, device=hip_device, requires_grad=True)
+    y = (x * p.grad).sum()        # keeps p.grad for its backward
+    clip_grad_norm_(p, 0.1)
+    with pytest.raises(RuntimeError):
+        y.backward()
+
+
+def test_side_stream_and_graph(hip_device):
+    from dogs_amd.gradclip import clip_grad_norm_
+    grads = _grads(hip_device, "many", seed=5)
+    params = _params(grads)
+    raw = [g.clone() for g in grads]
+    n = _norm(raw)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        a = clip_grad_norm_(params, n / 4)
+    side.synchronize()
+    assert abs(float(a) - n) <= 2 * U * n
+    clipped = [g.clone() for g in grads]
+    graphs = []
+    for limit in (n / 4, n / 2):                 # two graphs over the same gradients, each with its own workspace
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = clip_grad_norm_(params, limit)
+        graphs.append((graph, out))
+    for k in range(3):
+        for graph, out in graphs:
+            for g, r in zip(grads, raw):
+                g.copy_(r * (k + 1))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert abs(float(out) - _norm([r * (k + 1) for r in raw])) <= 2 * U * float(out)
+        for g, r in zip(grads, raw):
+            g.copy_(r)
+        graphs[0][0].replay()
+        assert all(torch.equal(g, c) for g, c in zip(grads, clipped))
+
+
+WIDTHS = (("xyz", (3,), 1.6e-4), ("f_dc", (1, 3), 2.5e-3), ("f_rest", (15, 3), 1.25e-4), ("opacity", (1,), 2.5e-2),
+          ("scaling", (3,), 5e-3), ("quaternion", (4,), 1e-3))
+
+
+def _scene(dev, n, seed):
+    from diff_gaussian_rasterization import SparseGaussianAdam
+    g = torch.Generator(device=dev).manual_seed(seed)
+    ps = [torch.nn.Parameter(torch.randn((n, *w), generator=g, device=dev)) for _, w, _ in WIDTHS]
+    opt = SparseGaussianAdam([{"params": [p], "lr": lr, "name": k} for p, (k, _, lr) in zip(ps, WIDTHS)], lr=0.0, eps=1e-15)
+    for p in ps:
+        p.grad = torch.randn(p.shape, generator=g, device=dev) * 1e-3
+        opt.state[p] = {"step": torch.tensor(0.0), "exp_avg": torch.randn(p.shape, generator=g, device=dev) * 1e-3,
+                        "exp_avg_sq": torch.rand(p.shape, generator=g, device=dev) * 1e-6 + 1e-10}
+    vis = torch.rand(n, generator=g, device=dev) < 0.6
+    return ps, opt, vis
+
+
+@pytest.mark.parametrize("n", [1, 777, 20011])
+@pytest.mark.parametrize("part", [0.3, 2.0])
+def test_clipped_step(hip_device, n, part):
+    """The clipped step has the bits of the plain step on gradients that were multiplied by the coefficient, and is the
+    formula in 64 bits: the moments within a few roundings of their terms, the step within those of its factors."""
+    from dogs_amd.gradclip import clip_coefficient
+    ps, opt, vis = _scene(hip_device, n, n)
+    qs, plain, _ = _scene(hip_device, n, n)
+    grads = [p.grad.clone() for p in ps]
+    total = _norm(grads)
+    before = [(p.detach().double(), opt.state[p]["exp_avg"].double(), opt.state[p]["exp_avg_sq"].double()) for p in ps]
+    norm = opt.step(vis, n, max_norm=part * total)
+    assert abs(float(norm) - total) <= 2 * U * total
+    assert all(torch.equal(p.grad, g) for p, g in zip(ps, grads))          # the gradients stay
+    _, coef = clip_coefficient(grads, part * total)
+    for q in qs:
+        q.grad = (q.grad.double() * coef).float()
+    assert plain.step(vis, n) is None
+    b1, b2 = float(np.float32(0.9)), float(np.float32(0.999))
+    c = min(1.0, part * total / (total + 1e-6))
+    for p, q, g, (p0, m0, v0), (_, _, lr) in zip(ps, qs, grads, before, WIDTHS):
+        for k in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(opt.state[p][k], plain.state[q][k])
+        assert torch.equal(p, q)
+        seen = vis.view(n, *[1] * (p.dim() - 1))
+        x = g.double() * c
+        m, v = b1 * m0 + (1 - b1) * x, b2 * v0 + (1 - b2) * x * x
+        dm = 6 * U * ((b1 * m0).abs() + ((1 - b1) * x).abs())
+        dv = 10 * U * v
+        step = lr * m / (v.sqrt() + 1e-15)
+        dp = lr * dm / v.sqrt() + step.abs() * 12 * U + 2 * U * p0.abs()
+        for got, want, tol, old in ((opt.state[p]["exp_avg"], m, dm, m0), (opt.state[p]["exp_avg_sq"], v, dv, v0),
+                                    (p.detach(), p0 - step, dp, p0)):
+            want, tol = torch.where(seen, want, old), torch.where(seen, tol, torch.zeros_like(tol))
+            assert bool(((got.double() - want).abs() <= tol).all())
+
+
+def test_clipped_step_with_statistics_and_missing_gradients(hip_device):
+    """Groups without a gradient stay out of norm and update; the densification statistics ride along unclipped."""
+    n = 500
+    ps, opt, vis = _scene(hip_device, n, 9)
+    ps[3].grad = None
+    keep = ps[3].detach().clone()
+    total = _norm([p.grad for p in ps if p.grad is not None])
+    stats = {"radii": torch.arange(n, dtype=torch.int32, device=hip_device), "dmeans2D": torch.ones((n, 3), device=hip_device),
+             "max_radii2D": torch.zeros(n, device=hip_device), "grad_accum": torch.zeros((n, 1), device=hip_device),
+             "denom": torch.zeros((n, 1), device=hip_device)}
+    norm = opt.step(vis, n, stats=stats, max_norm=total / 5)
+    assert abs(float(norm) - total) <= 2 * U * total
+    assert torch.equal(ps[3].detach(), keep)
+    assert torch.equal(stats["denom"].flatten(), vis.float())
+    assert torch.equal(stats["grad_accum"].flatten(), vis.float() * math.sqrt(2.0))
+    for p in ps:
+        p.grad = None
+    assert float(opt.step(vis, n, max_norm=1.0)) == 0.0
+
+
+def test_clipped_step_refusals(hip_device):
+    n = 40
+    ps, opt, vis = _scene(hip_device, n, 10)
+    z = {k: (torch.zeros_like(p), torch.zeros_like(p), 1.0) for p, (k, _, _) in zip(ps, WIDTHS)}
+    before = [p.detach().clone() for p in ps]
+    with pytest.raises(RuntimeError):
+        opt.step(vis, n, prox=z, max_norm=1.0)
+    for bad in (vis[:-1], vis[:1].expand(n + 1)):
+        with pytest.raises(RuntimeError):
+            opt.step(bad, n, max_norm=1.0)
+    with pytest.raises(RuntimeError):
+        opt.step(torch.ones(n + 1, dtype=torch.bool, device=hip_device), n + 1, max_norm=1.0)
+    with pytest.raises(RuntimeError):
+        opt.step(vis, n, max_norm=-1.0)
+    opt.state[ps[0]]["exp_avg"] = torch.zeros((n - 1, 3), device=hip_device)
+    with pytest.raises(RuntimeError):
+        opt.step(vis, n, max_norm=1.0)
+    assert all(torch.equal(p.detach(), b) for p, b in zip(ps, before))

@@ -1,0 +1,96 @@
+"""What embedding_lookup, grad_norm, clip_grad_norm_ and the library's entries below them refuse, without a GPU: every call
+here has to return an error before anything is launched."""
+import ctypes as C
+from array import array
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import os
+
+    from dogs_amd import _lib
+    from dogs_amd import build as B
+    if not os.path.exists(_lib.LIB_PATH):
+        B.build()
+    return _lib.load()
+
+
+def test_host_tensors_are_refused():
+    from dogs_amd.embedding import embedding_lookup
+    from dogs_amd.gradclip import clip_grad_norm_, grad_norm
+    with pytest.raises(RuntimeError):
+        embedding_lookup(torch.zeros(4, 4), torch.tensor([1]))
+    with pytest.raises(RuntimeError):
+        grad_norm([torch.ones(3)])
+    p = torch.nn.Parameter(torch.ones(3))
+    p.grad = torch.ones(3)
+    with pytest.raises(RuntimeError):
+        clip_grad_norm_([p], 1.0)
+
+
+def test_embedding_entry_refusals(lib):
+    def lookup(table=16, dtype=0, v=4, d=4, tokens=16, n=2, out=16):
+        return lib.dg_embedding_lookup(table, dtype, v, d, d, 1, tokens, 1, n, 1.0, out, None)
+    for kw in ({"dtype": 3}, {"dtype": -1}, {"v": 1 << 31}, {"n": 1 << 31}, {"d": 1 << 31}, {"table": None},
+               {"tokens": None}, {"out": None}):
+        assert lookup(**kw) != 0, kw
+    assert lookup(n=0) == 0 and lookup(d=0) == 0
+
+    def grad(g=16, dtype=0, v=4, d=4, tokens=16, n=2, out=16, scratch=256, nbytes=1 << 20):
+        return lib.dg_embedding_grad(g, dtype, tokens, 1, n, v, d, 1.0, -1, out, scratch, nbytes, None)
+    need = lib.dg_embedding_grad_scratch_bytes(4, 4, 2, 0)
+    for kw in ({"dtype": 3}, {"v": 1 << 31}, {"n": 1 << 31}, {"d": 1 << 31}, {"g": None}, {"tokens": None}, {"out": None},
+               {"scratch": None}, {"nbytes": need - 1}):
+        assert grad(**kw) != 0, kw
+    assert grad(v=0) == 0 and grad(d=0) == 0
+    assert lib.dg_embedding_grad_scratch_bytes(1 << 31, 4, 2, 0) == 0
+
+
+def test_gradient_entry_refusals(lib):
+    def args(ptrs, sizes, types):
+        keep = array("Q", ptrs), array("Q", sizes), array("B", types)
+        return keep, (len(ptrs), *[k.buffer_info()[0] for k in keep])
+    need = lib.dg_grad_norm_scratch_bytes(2)
+    for ptrs, sizes, types, text in (
+            ((4096, 4096), (10, 10), (0, 0), b"overlap"), ((4096, 4100), (10, 10), (0, 0), b"overlap"),
+            ((8192, 4096), (1, 1025), (0, 0), b"overlap"), ((4096, 8192), (2049, 1), (2, 2), b"overlap"),
+            ((4096, 8192), (1, 1), (0, 3), b"element type"), ((4096, 0), (1, 1), (0, 0), b"NULL"),
+            ((4096, 8194), (1, 1), (0, 0), b"aligned"), ((4096, 8193), (1, 1), (0, 2), b"aligned"),
+            ((4096, 8192), (1, 1 << 41), (0, 0), b"too large")):
+        keep, a = args(ptrs, sizes, types)
+        assert lib.dg_clip_grad_norm(*a, 2, 1.0, 256, 256, need, None) != 0
+        assert text in lib.dg_last_error(), (text, lib.dg_last_error())
+        assert lib.dg_grad_scale(*a, 256, None) != 0
+        del keep
+    keep, a = args((4096, 8192), (10, 10), (0, 0))
+    for order, limit, norm, scratch, nbytes in ((3, 1.0, 256, 256, need), (-1, 1.0, 256, 256, need), (2, -1.0, 256, 256, need),
+                                                (2, float("nan"), 256, 256, need), (2, 1.0, None, 256, need),
+                                                (2, 1.0, 256, None, need), (2, 1.0, 256, 256, need - 1)):
+        assert lib.dg_clip_grad_norm(*a, order, limit, norm, scratch, nbytes, None) != 0
+    assert lib.dg_grad_scale(*a, None, None) != 0
+    assert lib.dg_grad_norm(-1, None, None, None, 2, 1.0, 256, None, 256, need, None) != 0
+    assert lib.dg_grad_norm(2, None, None, None, 2, 1.0, 256, None, 256, need, None) != 0
+
+
+def test_appearance_batch_on_the_host():
+    """The batched module on the CPU equals its single views; a view that is there twice adds both gradients."""
+    from dogs_amd.masks import AppearanceEmbedding
+    torch.manual_seed(0)
+    net = AppearanceEmbedding(5).double()
+    with torch.no_grad():
+        net.appearance_embedding.normal_()
+    images = torch.rand((3, 3, 2, 3), dtype=torch.float64)
+    index = torch.tensor([4, 1, 4])
+    masks = net(images, index, (33, 50))
+    (masks ** 2).sum().backward()
+    got = net.appearance_embedding.grad.clone()
+    net.zero_grad()
+    one = torch.stack([net(images[k], int(index[k]), (33, 50)) for k in range(3)])
+    (one ** 2).sum().backward()
+    assert torch.allclose(masks, one, rtol=1e-12, atol=1e-12)
+    assert torch.allclose(got, net.appearance_embedding.grad, rtol=1e-9, atol=1e-12)
+    with pytest.raises(ValueError):
+        net(images, torch.tensor([4, 1]), (33, 50))
