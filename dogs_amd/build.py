@@ -18,7 +18,10 @@ ARCH = os.environ.get("DOGS_OFFLOAD_ARCH", "gfx950")
 # -ffp-contract=off + explicit fmaf and correctly rounded div/sqrt: the bit-exact key contract with the
 # CPU oracle (DESIGN.md "Bit-exact keys").
 FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-ffp-contract=off",
-         "-fhip-fp32-correctly-rounded-divide-sqrt", "-Wno-unused-result", "-munsafe-fp-atomics"]
+         "-fhip-fp32-correctly-rounded-divide-sqrt", "-Wno-unused-result", "-munsafe-fp-atomics",
+         # no packed fp32 instructions: some of their forms have given wrong results on this hardware now and then.  (The
+         # host pass warns that it does not know the feature.)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc() -> str:
