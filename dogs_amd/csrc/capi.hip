@@ -1195,7 +1195,8 @@ int dg_adam_update_groups_scaled(const dg_adam_group* groups, const dg_adam_prox
 
 static int embedding_sizes_ok(const char* what, int dtype, uint64_t V, uint32_t D, uint64_t n) {
     if (dtype < 0 || dtype > 2) return fail("%s: unknown element type %d", what, dtype);
-    if (V >= (1ull << 31) || n >= (1ull << 31) || D >= (1u << 31)) return fail("%s: V, n and D must be < 2^31%d", what);
+    if (V >= (1ull << 31) || n >= (1ull << 31) || D >= (1u << 23))
+        return fail("%s: V and n must be < 2^31, D < 2^23%d", what);
     return 0;
 }
 

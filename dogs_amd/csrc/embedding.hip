@@ -48,12 +48,376 @@ __global__ void __launch_bounds__(EB_THREADS) k_lookup(LookupArgs a, int lpr) {
     }
 }
 
-// the sort key of position i: its token, or V where it adds to no row
+// the row that position i adds to, or V where it adds to none
+__device__ __forceinline__ uint32_t key_at(const LookupGradArgs& a, uint32_t i) {
+    const int64_t t = token_at(a.tokens, a.wide, i);
+    return (t < 0 || t >= (int64_t)a.V || t == a.padding) ? a.V : (uint32_t)t;
+}
+
+// the lanes of the wave that hold the same `bits`-bit digit, among the active ones
+__device__ __forceinline__ uint64_t peers(uint32_t d, bool act, int bits) {
+    uint64_t m = __ballot(act);
+    for (int b = 0; b < bits; b++) {
+        const uint64_t s = __ballot((d >> b) & 1u);
+        m &= ((d >> b) & 1u) ? s : ~s;
+    }
+    return m;
+}
+// what the wave's lanes stored to LDS is what they load from here on (no barrier: one wave's accesses complete in order)
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+__device__ __forceinline__ uint64_t lanes_below() { return (1ull << (threadIdx.x & 63)) - 1ull; }
+
+// exclusive scan of one value per thread over the block; s_w holds a word per wave
+template <int NW>
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s_w) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    uint32_t x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 63) s_w[w] = x;
+    __syncthreads();
+    uint32_t off = 0;
+#pragma unroll
+    for (int k = 0; k < NW; k++) off += k < w ? s_w[k] : 0u;
+    return off + x - v;
+}
+
+// ---- sums over a sorted list
+//
+// A block holds a sorted stretch of (key, position) pairs in LDS and a slab of lpr x 16 bytes of the columns.  Its groups of
+// lpr lanes walk equal parts of the stretch, eight gradient rows in flight, and keep the running sum in registers;
+// a row whose entries lie within one part is stored from there.  Sums of runs that cross parts meet in LDS, in order, and
+// those that cross the block's ends go to the partials of the block: `head` for the run that began before it,
+// `tail` for the one that begins in it and goes on.  So a token that makes up half the batch costs no more than others.
+template <typename T> struct Cols {
+    typedef typename Vec<T>::type V;
+    static constexpr int W = Vec<T>::W;
+    uint32_t c0;     // first column of this lane
+    int nc;          // how many of its W columns exist
+    __device__ __forceinline__ V load(const T* row) const {
+        if (nc == W) return *reinterpret_cast<const V*>(row + c0);
+        V x = {};
+#pragma unroll
+        for (int j = 0; j < W; j++)
+            if (j < nc) x[j] = row[c0 + j];
+        return x;
+    }
+    __device__ __forceinline__ void store(T* row, const float (&acc)[W], float scale) const {
+        V x;
+#pragma unroll
+        for (int j = 0; j < W; j++) x[j] = (T)(acc[j] * scale);
+        if (nc == W) {
+            *reinterpret_cast<V*>(row + c0) = x;
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < W; j++)
+            if (j < nc) row[c0 + j] = x[j];
+    }
+    __device__ __forceinline__ void zero(T* row) const {
+        const float z[W] = {};
+        store(row, z, 0.0f);
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ Cols<T> cols_of(uint32_t slab, int lpr, uint32_t l, uint32_t D) {
+    const uint64_t c0 = ((uint64_t)slab * lpr + l) * Vec<T>::W;
+    const int64_t left = (int64_t)D - (int64_t)c0;
+    return {(uint32_t)c0, left >= Vec<T>::W ? Vec<T>::W : left > 0 ? (int)left : 0};
+}
+
+struct Stretch {
+    const uint32_t* key;     // LDS, ascending
+    const uint32_t* pos;     // LDS
+    uint32_t n;
+    bool open_front, open_back;   // the first / last run goes on outside
+    uint32_t row0;           // key k is row row0 + k of the table
+    float *head, *tail;      // the block's partials, D floats each (null: neither end is open)
+};
+
+constexpr int WALK = 8;
+
+// THREADS threads; s_part: LDS of THREADS * 2 * W floats
+template <typename T, int THREADS>
+__device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stretch& s, const Cols<T>& c, int lpr,
+                                            float* __restrict__ s_part) {
+    typedef typename Vec<T>::type V;
+    constexpr int W = Vec<T>::W;
+    const uint32_t groups = THREADS / lpr, g = threadIdx.x / lpr, part = (s.n + groups - 1) / groups;
+    const uint32_t lo = g * part < s.n ? g * part : s.n, hi = lo + part < s.n ? lo + part : s.n;
+    const T* grad = (const T*)a.grad;
+    T* table = (T*)a.dtable;
+    float* mine = s_part + threadIdx.x * (2 * W);   // this lane's columns of the group's head, then of its tail
+    if (lo < hi) {
+        const bool front = lo ? s.key[lo - 1] == s.key[lo] : s.open_front;
+        const bool back = hi < s.n ? s.key[hi] == s.key[hi - 1] : s.open_back;
+        float acc[W] = {};
+        uint32_t cur = s.key[lo];
+        bool first = true;
+        auto flush = [&](bool last) {
+            if (first && front) {
+#pragma unroll
+                for (int j = 0; j < W; j++) mine[j] = acc[j];
+            } else if (last && back) {
+#pragma unroll
+                for (int j = 0; j < W; j++) mine[W + j] = acc[j];
+            } else {
+                c.store(table + (uint64_t)(s.row0 + cur) * a.D, acc, a.scale);
+            }
+        };
+        for (uint32_t j0 = lo; j0 < hi; j0 += WALK) {
+            V x[WALK];
+            uint32_t k[WALK];
+#pragma unroll
+            for (int u = 0; u < WALK; u++) {
+                const uint32_t j = j0 + u < hi ? j0 + u : hi - 1;
+                k[u] = s.key[j];
+                x[u] = c.load(grad + (uint64_t)s.pos[j] * a.D);
+            }
+#pragma unroll
+            for (int u = 0; u < WALK; u++) {
+                if (j0 + u >= hi) break;
+                if (k[u] != cur) {
+                    flush(false);
+                    first = false;
+                    cur = k[u];
+#pragma unroll
+                    for (int j = 0; j < W; j++) acc[j] = 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < W; j++) acc[j] += (float)x[u][j];
+            }
+        }
+        flush(true);
+    }
+    __syncthreads();
+    if (lo >= hi) return;
+    // the group whose tail begins a run joins it with the heads after it; group 0 also joins the run that was open in front
+    const uint32_t lane_off = (threadIdx.x - g * lpr) * (2 * W);
+    auto join = [&](float (&acc)[W], uint32_t k, uint32_t h) {   // heads of parts h, h + 1, ... while they hold key k
+        for (; h < groups && h * part < s.n && s.key[h * part] == k; h++) {
+            const float* o = s_part + (uint64_t)h * lpr * (2 * W) + lane_off;
+#pragma unroll
+            for (int j = 0; j < W; j++) acc[j] += o[j];
+        }
+    };
+    auto put = [&](float* dst, const float (&acc)[W]) {
+#pragma unroll
+        for (int j = 0; j < W; j++)
+            if (j < c.nc) dst[c.c0 + j] = acc[j];
+    };
+    if (g == 0 && s.open_front) {
+        float acc[W];
+#pragma unroll
+        for (int j = 0; j < W; j++) acc[j] = mine[j];
+        join(acc, s.key[0], 1);
+        put(s.head, acc);
+    }
+    const uint32_t k = s.key[hi - 1];
+    const bool begins = lo ? s.key[lo - 1] != k : !(s.open_front && s.key[0] == k);
+    const bool goes_on = hi < s.n ? s.key[hi] == k : s.open_back;
+    if (begins && goes_on) {
+        float acc[W];
+#pragma unroll
+        for (int j = 0; j < W; j++) acc[j] = mine[W + j];
+        join(acc, k, g + 1);
+        if (s.open_back && s.key[s.n - 1] == k) put(s.tail, acc);
+        else c.store(table + (uint64_t)(s.row0 + k) * a.D, acc, a.scale);
+    }
+}
+
+// ---- few tokens: one launch
+//
+// A block owns `rows` (a power of two, up to 256) rows of the table and one slab of columns.  It looks through all tokens,
+// each wave through a contiguous part of them, ranks those of its rows (stable counting sort by row, in LDS), and sums.
+template <typename T, int NW>
+__global__ void __launch_bounds__(NW * 64) k_grad_small(LookupGradArgs a, int lpr, uint32_t rows, int row_bits, uint32_t slabs) {
+    constexpr int IT = 16, CAP = NW * 64 * IT;
+    __shared__ uint32_t s_key[CAP], s_pos[CAP];
+    __shared__ uint32_t s_hist[NW][256];
+    __shared__ uint32_t s_w[NW];
+    __shared__ float s_part[NW * 64 * 2 * Vec<T>::W];
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+    const uint32_t v0 = (uint32_t)(blockIdx.x / slabs) * rows, slab = blockIdx.x % slabs;
+    const uint32_t nrows = a.V - v0 < rows ? a.V - v0 : rows;
+    for (int i = t; i < NW * 256; i += NW * 64) (&s_hist[0][0])[i] = 0u;
+    uint32_t code[IT];   // row << 16 | rank among this wave's tokens of the row
+    const uint32_t base = (uint32_t)w * (64 * IT) + lane;
+#pragma unroll
+    for (int r = 0; r < IT; r++) {
+        const uint32_t i = base + 64 * r;
+        code[r] = i < a.n ? key_at(a, i) - v0 : ~0u;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < IT; r++) {
+        const uint32_t lr = code[r];
+        const bool act = lr < nrows;
+        code[r] = ~0u;
+        if (!__ballot(act)) continue;
+        const uint64_t m = peers(lr, act, row_bits);
+        const uint32_t before = (uint32_t)__popcll(m & lanes_below());
+        if (act) {
+            const uint32_t had = s_hist[w][lr];
+            code[r] = lr << 16 | (had + before);
+            if (!(m >> lane >> 1)) s_hist[w][lr] = had + before + 1;   // the last peer publishes the count
+        }
+        wave_lds_fence();
+    }
+    __syncthreads();
+    uint32_t mine = 0;
+    if (t < 256)
+        for (int k = 0; k < NW; k++) mine += s_hist[k][t];
+    uint32_t at = block_scan<NW>(mine, s_w);
+    uint32_t total = 0;
+    for (int k = 0; k < NW; k++) total += s_w[k];
+    if (t < 256)
+        for (int k = 0; k < NW; k++) {
+            const uint32_t n = s_hist[k][t];
+            s_hist[k][t] = at;
+            at += n;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < IT; r++) {
+        if (code[r] == ~0u) continue;
+        const uint32_t lr = code[r] >> 16, o = s_hist[w][lr] + (code[r] & 0xffffu);
+        s_key[o] = lr;
+        s_pos[o] = base + 64 * r;
+    }
+    __syncthreads();
+    const Cols<T> c = cols_of<T>(slab, lpr, t & (lpr - 1), a.D);
+    // rows without a token: the last wave's start of row r, advanced past its tokens, is where row r + 1 begins
+    for (uint32_t r = t / lpr; r < nrows; r += NW * 64 / lpr) {
+        const uint32_t end = r + 1 < 256 ? s_hist[0][r + 1] : total;
+        if (s_hist[0][r] == end) c.zero((T*)a.dtable + (uint64_t)(v0 + r) * a.D);
+    }
+    const Stretch s = {s_key, s_pos, total, false, false, v0, nullptr, nullptr};
+    sum_stretch<T, NW * 64>(a, s, c, lpr, s_part);
+}
+
+// ---- many tokens: sort them, sum stretches of the sorted list, join what crosses stretches
+
+// Stable radix sort of (key, position), digits of `bits` bits, 1024 pairs per block: the launches are latency, so
+// the digits are as wide as two passes need (up to 11 bits) and a pass is spread over more blocks than a sort of
+// millions would take.
+constexpr int TS_THREADS = 256, TS_IT = 4, TS_TILE = TS_THREADS * TS_IT, TS_MAX_BITS = 11;
+constexpr uint32_t TS_MAX_N = 1u << 18;   // 256 tiles: the scan of a digit's counts over tiles is one block wide
+
+__device__ __forceinline__ uint32_t sort_key(const LookupGradArgs& a, const uint32_t* keys, uint32_t i) {
+    return keys ? keys[i] : key_at(a, i);
+}
+
+__global__ void __launch_bounds__(TS_THREADS) k_sort_count(LookupGradArgs a, const uint32_t* __restrict__ keys, int shift,
+                                                           int bits, uint32_t* __restrict__ counts) {
+    __shared__ uint32_t hist[1 << TS_MAX_BITS];
+    const uint32_t bins = 1u << bits, base = blockIdx.x * TS_TILE + threadIdx.x;
+    uint32_t k[TS_IT];
+#pragma unroll
+    for (int r = 0; r < TS_IT; r++) {
+        const uint32_t i = base + r * TS_THREADS;
+        k[r] = i < a.n ? sort_key(a, keys, i) : 0u;
+    }
+    for (uint32_t d = threadIdx.x; d < bins; d += TS_THREADS) hist[d] = 0u;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < TS_IT; r++)
+        if (base + r * TS_THREADS < a.n) atomicAdd(&hist[(k[r] >> shift) & (bins - 1)], 1u);
+    __syncthreads();
+    for (uint32_t d = threadIdx.x; d < bins; d += TS_THREADS) counts[(uint64_t)d * gridDim.x + blockIdx.x] = hist[d];
+}
+
+// block d: the exclusive scan of digit d's counts over the tiles, and its total
+__global__ void __launch_bounds__(TS_THREADS) k_sort_scan(uint32_t* __restrict__ counts, uint32_t tiles,
+                                                          uint32_t* __restrict__ totals) {
+    __shared__ uint32_t s_w[TS_THREADS / 64];
+    uint32_t* c = counts + (uint64_t)blockIdx.x * tiles;
+    const uint32_t v = threadIdx.x < tiles ? c[threadIdx.x] : 0u;
+    const uint32_t x = block_scan<TS_THREADS / 64>(v, s_w);
+    if (threadIdx.x < tiles) c[threadIdx.x] = x;
+    if (threadIdx.x == TS_THREADS - 1) totals[blockIdx.x] = x + v;
+}
+
+__global__ void __launch_bounds__(TS_THREADS) k_sort_scatter(LookupGradArgs a, const uint32_t* __restrict__ keys,
+                                                             const uint32_t* __restrict__ pos, int shift, int bits,
+                                                             const uint32_t* __restrict__ counts,
+                                                             const uint32_t* __restrict__ totals,
+                                                             uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out) {
+    constexpr int NW = TS_THREADS / 64, PER = (1 << TS_MAX_BITS) / TS_THREADS;
+    __shared__ uint32_t hist[NW][1 << TS_MAX_BITS];
+    __shared__ uint32_t s_w[NW];
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+    const uint32_t bins = 1u << bits, base = blockIdx.x * TS_TILE + w * (64 * TS_IT) + lane;
+    uint32_t k[TS_IT], p[TS_IT], rank[TS_IT];
+#pragma unroll
+    for (int r = 0; r < TS_IT; r++) {
+        const uint32_t i = base + 64 * r;
+        k[r] = i < a.n ? sort_key(a, keys, i) : 0u;
+        p[r] = i < a.n && pos ? pos[i] : i;
+    }
+    // bins of a thread are neighbours, so one scan over the threads orders the digits
+    const uint32_t per = bins > TS_THREADS ? bins / TS_THREADS : 1u;
+    uint32_t tot[PER], before[PER], sum = 0;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const uint32_t d = t * per + j;
+        const bool in = (uint32_t)j < per && d < bins;
+        tot[j] = in ? totals[d] : 0u;
+        before[j] = in ? counts[(uint64_t)d * gridDim.x + blockIdx.x] : 0u;
+        sum += tot[j];
+    }
+    for (uint32_t d = t; d < bins; d += TS_THREADS)
+#pragma unroll
+        for (int q = 0; q < NW; q++) hist[q][d] = 0u;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < TS_IT; r++) {
+        const bool act = base + 64 * r < a.n;
+        const uint32_t d = (k[r] >> shift) & (bins - 1);
+        const uint64_t m = peers(d, act, bits);
+        const uint32_t lower = (uint32_t)__popcll(m & lanes_below());
+        if (act) {
+            const uint32_t had = hist[w][d];
+            rank[r] = had + lower;
+            if (!(m >> lane >> 1)) hist[w][d] = had + lower + 1;
+        }
+        wave_lds_fence();
+    }
+    uint32_t start = block_scan<NW>(sum, s_w);   // its barrier is also the one after the ranking
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const uint32_t d = t * per + j;
+        if ((uint32_t)j >= per || d >= bins) continue;
+        uint32_t at = start + before[j];
+        start += tot[j];
+#pragma unroll
+        for (int q = 0; q < NW; q++) {
+            const uint32_t n = hist[q][d];
+            hist[q][d] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < TS_IT; r++) {
+        if (base + 64 * r >= a.n) continue;
+        const uint32_t o = hist[w][(k[r] >> shift) & (bins - 1)] + rank[r];
+        keys_out[o] = k[r];
+        pos_out[o] = p[r];
+    }
+}
+
 __global__ void __launch_bounds__(EB_THREADS) k_keys(LookupGradArgs a, uint32_t* __restrict__ keys) {
     const uint32_t i = blockIdx.x * EB_THREADS + threadIdx.x;
-    if (i >= a.n) return;
-    const int64_t t = token_at(a.tokens, a.wide, i);
-    keys[i] = (t < 0 || t >= (int64_t)a.V || t == a.padding) ? a.V : (uint32_t)t;
+    if (i < a.n) keys[i] = key_at(a, i);
 }
 
 __device__ __forceinline__ uint32_t lower_bound(const uint32_t* __restrict__ keys, uint32_t n, uint32_t v) {
@@ -65,23 +429,102 @@ __device__ __forceinline__ uint32_t lower_bound(const uint32_t* __restrict__ key
     return lo;
 }
 
-// a block per table row: the sum of its token's gradient rows, in their order
+struct SumPlan {
+    const uint32_t *keys, *pos;
+    float* partial;          // [stretches][2][D]: head, tail
+    uint32_t stretches, entries;   // entries of a stretch
+    uint32_t slabs;
+    uint32_t zero_rows;      // rows of a block that clears rows without a token
+    int lpr;
+};
+constexpr uint32_t MAX_ENTRIES = 2048;
+
+// blocks [0, stretches * slabs): the sums; the rest: zeros in the rows that no token names
 template <typename T>
-__global__ void __launch_bounds__(EB_THREADS) k_rows(LookupGradArgs a, const uint32_t* __restrict__ keys,
-                                                     const uint32_t* __restrict__ pos) {
-    __shared__ uint32_t range[2];
-    for (uint64_t v = blockIdx.x; v < a.V; v += gridDim.x) {
-        __syncthreads();
-        if (threadIdx.x < 2) range[threadIdx.x] = lower_bound(keys, a.n, (uint32_t)v + threadIdx.x);
-        __syncthreads();
-        const uint32_t lo = range[0], hi = range[1];
-        T* out = (T*)a.dtable + v * a.D;
-        for (uint32_t c = threadIdx.x; c < a.D; c += EB_THREADS) {
-            float acc = 0.0f;
-            for (uint32_t j = lo; j < hi; j++) acc += (float)((const T*)a.grad)[(uint64_t)pos[j] * a.D + c];
-            out[c] = (T)(acc * a.scale);
+__global__ void __launch_bounds__(EB_THREADS) k_grad_sums(LookupGradArgs a, SumPlan p) {
+    __shared__ uint32_t s_key[MAX_ENTRIES], s_pos[MAX_ENTRIES];
+    __shared__ float s_part[EB_THREADS * 2 * Vec<T>::W];
+    const uint32_t l = threadIdx.x & (p.lpr - 1);
+    const uint64_t sums = (uint64_t)p.stretches * p.slabs;
+    if (blockIdx.x < sums) {
+        const uint32_t c = blockIdx.x / p.slabs, slab = blockIdx.x % p.slabs;
+        const uint32_t e0 = c * p.entries, e1 = e0 + p.entries < a.n ? e0 + p.entries : a.n;
+        for (uint32_t j = threadIdx.x; j < e1 - e0; j += EB_THREADS) {
+            s_key[j] = p.keys[e0 + j];
+            s_pos[j] = p.pos[e0 + j];
         }
+        const uint32_t before = e0 ? p.keys[e0 - 1] : a.V, after = e1 < a.n ? p.keys[e1] : a.V;
+        __syncthreads();
+        uint32_t n = e1 - e0;
+        if (s_key[n - 1] == a.V) n = lower_bound(s_key, n, a.V);   // entries that add to no row are last
+        if (!n) return;
+        float* part = p.partial + (uint64_t)c * 2 * a.D;
+        const Stretch s = {s_key, s_pos, n, before == s_key[0], n == e1 - e0 && after == s_key[n - 1], 0, part, part + a.D};
+        sum_stretch<T, EB_THREADS>(a, s, cols_of<T>(slab, p.lpr, l, a.D), p.lpr, s_part);
+        return;
     }
+    const uint64_t v0 = (blockIdx.x - sums) * p.zero_rows;
+    for (uint32_t r = threadIdx.x; r < p.zero_rows; r += EB_THREADS) {
+        const uint64_t v = v0 + r;
+        uint32_t empty = 0;
+        if (v < a.V) {
+            const uint32_t at = lower_bound(p.keys, a.n, (uint32_t)v);
+            empty = at == a.n || p.keys[at] != (uint32_t)v;
+        }
+        s_key[r] = empty;
+    }
+    __syncthreads();
+    const uint32_t groups = EB_THREADS / p.lpr;
+    for (uint32_t r = threadIdx.x / p.lpr; r < p.zero_rows; r += groups)
+        if (s_key[r])
+            for (uint32_t slab = 0; slab < p.slabs; slab++)
+                cols_of<T>(slab, p.lpr, l, a.D).zero((T*)a.dtable + (v0 + r) * a.D);
+}
+
+// The runs that cross stretches: the block of the stretch where one begins adds the tail there and the heads after it, a
+// quarter of them per wave, in order.
+template <typename T>
+__global__ void __launch_bounds__(EB_THREADS) k_grad_join(LookupGradArgs a, SumPlan p) {
+    __shared__ float4 s[EB_THREADS];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const uint32_t c = blockIdx.x, e0 = c * p.entries, e1 = e0 + p.entries;   // never the last stretch: e1 < n
+    const uint32_t k = p.keys[e1 - 1];
+    if (k == a.V || p.keys[e1] != k || (e0 && p.keys[e0 - 1] == k)) return;
+    uint32_t heads = 0;   // stretches after c that begin with k
+    for (bool more = true; more;) {
+        const uint64_t h = (uint64_t)c + 1 + heads + lane;
+        const uint64_t same = __ballot(h < p.stretches && p.keys[(uint32_t)(h * p.entries)] == k);
+        more = same == ~0ull;
+        heads += more ? 64u : (uint32_t)__builtin_ctzll(~same);
+    }
+    const uint32_t per = (heads + 3) / 4, lo = w * per < heads ? w * per : heads, hi = lo + per < heads ? lo + per : heads;
+    const uint64_t c0 = (uint64_t)blockIdx.y * 256 + 4 * lane;
+    float acc[4] = {};
+    const float* base = p.partial + (uint64_t)c * 2 * a.D;
+    typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
+    const int nc = c0 + 4 <= a.D ? 4 : c0 < a.D ? (int)(a.D - c0) : 0;
+    auto add = [&](const float* row) {
+        if (nc == 4) {
+            const F4 x = *reinterpret_cast<const F4*>(row + c0);
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[j] += x[j];
+        } else {
+            for (int j = 0; j < nc; j++) acc[j] += row[c0 + j];
+        }
+    };
+    if (w == 0) add(base + a.D);
+#pragma unroll 8
+    for (uint32_t h = lo; h < hi; h++) add(base + (uint64_t)(h + 1) * 2 * a.D);
+    s[threadIdx.x] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int q = 1; q < 4; q++) {
+        const float4 x = s[q * 64 + lane];
+        acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
+    }
+    T* out = (T*)a.dtable + (uint64_t)k * a.D + c0;
+    for (int j = 0; j < nc; j++) out[j] = (T)(acc[j] * a.scale);
 }
 
 inline size_t pad(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -106,25 +549,113 @@ void launch_embedding_lookup(const LookupArgs& a, int dtype, hipStream_t s) {
     else k_lookup<__bf16><<<blocks, EB_THREADS, 0, s>>>(a, lpr);
 }
 
+namespace {
+
+// lanes of a row's slab: as many 16-byte pieces as the row has, up to a wave
+int lanes_per_row(uint32_t D, int dtype, int most) {
+    const uint32_t W = 16 / elem_bytes(dtype), pieces = (D + W - 1) / W;
+    int lpr = 1;
+    while (lpr < most && (uint32_t)lpr < pieces) lpr <<= 1;
+    return lpr;
+}
+uint32_t slabs_of(uint32_t D, int dtype, int lpr) {
+    const uint32_t per = lpr * (16 / elem_bytes(dtype));
+    return (D + per - 1) / per;
+}
+
+constexpr uint32_t SMALL_N = 4096;   // as many tokens as the one-launch kernel holds
+
+SumPlan plan_of(const LookupGradArgs& a, int dtype) {
+    SumPlan p = {};
+    p.lpr = lanes_per_row(a.D, dtype, 64);
+    p.slabs = slabs_of(a.D, dtype, p.lpr);
+    const uint32_t groups = EB_THREADS / p.lpr;
+    p.entries = 32 * groups < MAX_ENTRIES ? 32 * groups : MAX_ENTRIES;
+    p.stretches = (a.n + p.entries - 1) / p.entries;
+    const uint64_t row = (uint64_t)a.D * elem_bytes(dtype);
+    p.zero_rows = row >= 32768 ? 1u : (uint32_t)(32768 / row < 256 ? 32768 / row : 256);
+    return p;
+}
+
+// [keys, pos] twice, the sort's counts, the partials
+struct GradScratch {
+    size_t pair, counts, partial, bytes;
+};
+GradScratch scratch_of(const LookupGradArgs& a, const SumPlan& p) {
+    GradScratch s;
+    s.pair = pad(4 * (size_t)a.n);
+    s.counts = 4 * s.pair;
+    const size_t tiles = ((size_t)a.n + TS_TILE - 1) / TS_TILE;
+    const size_t counts = a.n <= TS_MAX_N ? 4 * ((size_t)1 << TS_MAX_BITS) * (tiles + 1) : radix_sort_temp_bytes(a.n);
+    s.partial = s.counts + pad(counts);
+    s.bytes = s.partial + (size_t)p.stretches * 2 * a.D * 4;
+    return s;
+}
+
+template <typename T>
+void grad_small(const LookupGradArgs& a, int dtype, hipStream_t s) {
+    const int lpr = lanes_per_row(a.D, dtype, 64);
+    const uint32_t slabs = slabs_of(a.D, dtype, lpr);
+    uint32_t rows = 1;
+    int bits = 0;
+    while (rows < 256 && (uint64_t)((a.V + rows - 1) / rows) * slabs > 1024) { rows <<= 1; bits++; }
+    const uint64_t blocks = (uint64_t)((a.V + rows - 1) / rows) * slabs;
+    k_grad_small<T, 4><<<(uint32_t)blocks, 256, 0, s>>>(a, lpr, rows, bits, slabs);
+}
+
+template <typename T>
+void grad_sums(const LookupGradArgs& a, const SumPlan& p, hipStream_t s) {
+    const uint64_t blocks = (uint64_t)p.stretches * p.slabs + ((uint64_t)a.V + p.zero_rows - 1) / p.zero_rows;
+    k_grad_sums<T><<<(uint32_t)blocks, EB_THREADS, 0, s>>>(a, p);
+    if (p.stretches > 1) k_grad_join<T><<<dim3(p.stretches - 1, (a.D + 255) / 256), EB_THREADS, 0, s>>>(a, p);
+}
+
+}  // namespace
+
 size_t embedding_grad_scratch_bytes(uint32_t V, uint32_t D, uint32_t n, int dtype) {
-    (void)V; (void)D; (void)dtype;
-    return n ? 4 * pad(4 * (size_t)n) + pad(radix_sort_temp_bytes(n)) : 256;
+    if (n <= SMALL_N) return 256;
+    LookupGradArgs a = {};
+    a.V = V; a.D = D; a.n = n;
+    return scratch_of(a, plan_of(a, dtype)).bytes;
 }
 
 void launch_embedding_grad(const LookupGradArgs& a, int dtype, void* scratch, hipStream_t s) {
-    char* b = (char*)scratch;
-    const size_t step = pad(4 * (size_t)a.n);
-    uint32_t *k0 = (uint32_t*)b, *v0 = (uint32_t*)(b + step), *k1 = (uint32_t*)(b + 2 * step), *v1 = (uint32_t*)(b + 3 * step);
-    int which = 0;
-    if (a.n) {
-        k_keys<<<(uint32_t)(((uint64_t)a.n + EB_THREADS - 1) / EB_THREADS), EB_THREADS, 0, s>>>(a, k0);
-        which = radix_sort_pairs(k0, v0, k1, v1, nullptr, a.n, 0, key_bits(a.V), b + 4 * step, s);
+    if (a.n <= SMALL_N) {
+        if (dtype == 0) grad_small<float>(a, dtype, s);
+        else if (dtype == 1) grad_small<_Float16>(a, dtype, s);
+        else grad_small<__bf16>(a, dtype, s);
+        return;
     }
-    const uint32_t *keys = which ? k1 : k0, *pos = which ? v1 : v0;
-    const uint32_t blocks = a.V < EB_MAX_BLOCKS ? a.V : EB_MAX_BLOCKS;
-    if (dtype == 0) k_rows<float><<<blocks, EB_THREADS, 0, s>>>(a, keys, pos);
-    else if (dtype == 1) k_rows<_Float16><<<blocks, EB_THREADS, 0, s>>>(a, keys, pos);
-    else k_rows<__bf16><<<blocks, EB_THREADS, 0, s>>>(a, keys, pos);
+    SumPlan p = plan_of(a, dtype);
+    const GradScratch o = scratch_of(a, p);
+    char* b = (char*)scratch;
+    uint32_t *k[2], *v[2];
+    for (int q = 0; q < 2; q++) {
+        k[q] = (uint32_t*)(b + 2 * q * o.pair);
+        v[q] = (uint32_t*)(b + (2 * q + 1) * o.pair);
+    }
+    int in = 0;
+    const int bits = key_bits(a.V);
+    if (a.n <= TS_MAX_N) {
+        const uint32_t tiles = (a.n + TS_TILE - 1) / TS_TILE;
+        uint32_t *counts = (uint32_t*)(b + o.counts), *totals = counts + ((size_t)tiles << TS_MAX_BITS);
+        const int passes = (bits + TS_MAX_BITS - 1) / TS_MAX_BITS, digit = (bits + passes - 1) / passes;
+        for (int q = 0; q < passes; q++, in ^= 1) {
+            const uint32_t *ki = q ? k[in] : nullptr, *vi = q ? v[in] : nullptr;
+            k_sort_count<<<tiles, TS_THREADS, 0, s>>>(a, ki, q * digit, digit, counts);
+            k_sort_scan<<<1u << digit, TS_THREADS, 0, s>>>(counts, tiles, totals);
+            k_sort_scatter<<<tiles, TS_THREADS, 0, s>>>(a, ki, vi, q * digit, digit, counts, totals, k[in ^ 1], v[in ^ 1]);
+        }
+    } else {
+        k_keys<<<(uint32_t)(((uint64_t)a.n + EB_THREADS - 1) / EB_THREADS), EB_THREADS, 0, s>>>(a, k[0]);
+        in = radix_sort_pairs(k[0], v[0], k[1], v[1], nullptr, a.n, 0, bits, b + o.counts, s);
+    }
+    p.keys = k[in];
+    p.pos = v[in];
+    p.partial = (float*)(b + o.partial);
+    if (dtype == 0) grad_sums<float>(a, p, s);
+    else if (dtype == 1) grad_sums<_Float16>(a, p, s);
+    else grad_sums<__bf16>(a, p, s);
 }
 
 }  // namespace gs

@@ -239,7 +239,7 @@ enum { DG_F32 = 0, DG_F16 = 1, DG_BF16 = 2 };   /* element types */
 
 /* out [n][D] = scale * table[tokens[i]], in table's type (products in 32 bits, rounded once).  table: V rows of D elements,
  * element (v, c) at v * row_stride + c * col_stride (in elements); tokens: n of 32 or (wide) 64 bits.  A token outside
- * [0, V) reads nothing and its row of out is NaN.  n, V < 2^31. */
+ * [0, V) reads nothing and its row of out is NaN.  n, V < 2^31, D < 2^23. */
 int dg_embedding_lookup(const void* table, int dtype, uint64_t V, uint32_t D, int64_t row_stride, int64_t col_stride,
                         const void* tokens, int wide, uint64_t n, float scale, void* out, dg_stream_t stream);
 /* Its gradient for the table: dtable [V][D] (every element is written) = scale * sum of the rows i of grad [n][D] with

@@ -34,7 +34,7 @@ def test_host_tensors_are_refused():
 def test_embedding_entry_refusals(lib):
     def lookup(table=16, dtype=0, v=4, d=4, tokens=16, n=2, out=16):
         return lib.dg_embedding_lookup(table, dtype, v, d, d, 1, tokens, 1, n, 1.0, out, None)
-    for kw in ({"dtype": 3}, {"dtype": -1}, {"v": 1 << 31}, {"n": 1 << 31}, {"d": 1 << 31}, {"table": None},
+    for kw in ({"dtype": 3}, {"dtype": -1}, {"v": 1 << 31}, {"n": 1 << 31}, {"d": 1 << 23}, {"table": None},
                {"tokens": None}, {"out": None}):
         assert lookup(**kw) != 0, kw
     assert lookup(n=0) == 0 and lookup(d=0) == 0
@@ -42,7 +42,7 @@ def test_embedding_entry_refusals(lib):
     def grad(g=16, dtype=0, v=4, d=4, tokens=16, n=2, out=16, scratch=256, nbytes=1 << 20):
         return lib.dg_embedding_grad(g, dtype, tokens, 1, n, v, d, 1.0, -1, out, scratch, nbytes, None)
     need = lib.dg_embedding_grad_scratch_bytes(4, 4, 2, 0)
-    for kw in ({"dtype": 3}, {"v": 1 << 31}, {"n": 1 << 31}, {"d": 1 << 31}, {"g": None}, {"tokens": None}, {"out": None},
+    for kw in ({"dtype": 3}, {"v": 1 << 31}, {"n": 1 << 31}, {"d": 1 << 23}, {"g": None}, {"tokens": None}, {"out": None},
                {"scratch": None}, {"nbytes": need - 1}):
         assert grad(**kw) != 0, kw
     assert grad(v=0) == 0 and grad(d=0) == 0
