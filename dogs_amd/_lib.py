@@ -370,6 +370,9 @@ def stream_of(device: torch.device):
 
 
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# the current device without torch.cuda.current_device()'s initialisation check (0.2 us instead of 1 us, 4 us on an autograd
+# thread); a HIP tensor exists wherever device_ctx is used
+_GET_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 _SAME_DEVICE = contextlib.nullcontext()
@@ -378,7 +381,7 @@ _SAME_DEVICE = contextlib.nullcontext()
 def device_ctx(device: torch.device):
     """torch.cuda.device(device), or a no-op when it is already the current device (the usual case: entering and
     leaving the context costs a few us per call)."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == _GET_DEVICE():
         return _SAME_DEVICE
     return torch.cuda.device(device)
 

@@ -1223,9 +1223,9 @@ int dg_embedding_grad(const void* grad, int dtype, const void* tokens, int wide,
     API_GUARD();
     if (embedding_sizes_ok("embedding_grad", dtype, V, D, n)) return 1;
     if (V == 0 || D == 0) return 0;
-    if ((n && (!grad || !tokens)) || !dtable || !scratch) return fail("embedding_grad: a tensor is NULL%s%d");
-    if (scratch_bytes < gs::embedding_grad_scratch_bytes((uint32_t)V, D, (uint32_t)n, dtype))
-        return fail("embedding_grad: scratch too small%s%d");
+    if ((n && (!grad || !tokens)) || !dtable) return fail("embedding_grad: a tensor is NULL%s%d");
+    const size_t need = gs::embedding_grad_scratch_bytes((uint32_t)V, D, (uint32_t)n, dtype);
+    if (need && (!scratch || scratch_bytes < need)) return fail("embedding_grad: scratch missing or too small%s%d");
     gs::LookupGradArgs a = {grad, tokens, wide != 0, (uint32_t)n, D, (uint32_t)V, scale, padding, dtable};
     gs::launch_embedding_grad(a, dtype, scratch, (hipStream_t)stream);
     HIP_OK(hipGetLastError());

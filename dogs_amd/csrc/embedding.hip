@@ -613,7 +613,7 @@ void grad_sums(const LookupGradArgs& a, const SumPlan& p, hipStream_t s) {
 }  // namespace
 
 size_t embedding_grad_scratch_bytes(uint32_t V, uint32_t D, uint32_t n, int dtype) {
-    if (n <= SMALL_N) return 256;
+    if (n <= SMALL_N) return 0;
     LookupGradArgs a = {};
     a.V = V; a.D = D; a.n = n;
     return scratch_of(a, plan_of(a, dtype)).bytes;

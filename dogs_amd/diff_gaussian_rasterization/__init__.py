@@ -248,10 +248,10 @@ def _clip(groups, visibility, N, max_norm):
     from ..gradclip import clip_coefficient
     if visibility.numel() != N:
         raise RuntimeError(f"step: visibility has {visibility.numel()} entries for {N} rows")
-    for param, grad, m, v, _, _ in groups:
-        _C._check_group(param, grad, m, v)
-        if param.device != visibility.device or any(t.device != param.device or t.numel() != param.numel()
-                                                    for t in (grad, m, v)) or (param.numel() % N if N else param.numel()):
+    index = visibility.get_device()
+    for group in groups:
+        n = group[0].numel()
+        if any(t.numel() != n or t.get_device() != index for t in group[:4]) or (n % N if N else n):
             raise RuntimeError(f"step: a group's tensors are not {N} rows each on {visibility.device}")
     if not groups:
         return torch.zeros((), device=visibility.device), None

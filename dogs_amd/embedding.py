@@ -18,36 +18,46 @@ _WIDE = {torch.int64: 1, torch.int32: 0}
 
 def _lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float) -> torch.Tensor:
     v, d = table.shape
-    out = torch.empty((*tokens.shape, d), dtype=table.dtype, device=table.device)
-    with _lib.device_ctx(table.device):
+    device = table.device
+    out = table.new_empty((*tokens.shape, d))
+    with _lib.device_ctx(device):
         _lib.check(_lib.load().dg_embedding_lookup(table.data_ptr(), _DTYPES[table.dtype], v, d, *table.stride(),
                                                    tokens.data_ptr(), _WIDE[tokens.dtype], tokens.numel(), scale,
-                                                   out.data_ptr(), _lib.stream_of(table.device)))
+                                                   out.data_ptr(), _lib.stream_of(device)))
     return out
+
+
+def _table_grad(ctx, g):
+    tokens, = ctx.saved_tensors
+    v, d, scale, padding = ctx.call
+    g = g.contiguous()
+    device, dtype, n = g.device, _DTYPES[g.dtype], tokens.numel()
+    L = _lib.load()
+    dtable = g.new_empty((v, d))
+    nbytes = L.dg_embedding_grad_scratch_bytes(v, d, n, dtype)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    with _lib.device_ctx(device):
+        _lib.check(L.dg_embedding_grad(g.data_ptr(), dtype, tokens.data_ptr(), _WIDE[tokens.dtype], n, v, d, scale, padding,
+                                       dtable.data_ptr(), scratch.data_ptr() if nbytes else None, nbytes,
+                                       _lib.stream_of(device)))
+    return dtable, None, None, None
 
 
 class _EmbeddingLookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, tokens, scale, padding):
         ctx.save_for_backward(tokens)
-        ctx.sizes, ctx.dtype, ctx.scale, ctx.padding = table.shape, table.dtype, scale, padding
+        ctx.call = (*table.shape, scale, padding)
         return _lookup(table, tokens, scale)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        tokens, = ctx.saved_tensors
-        (v, d), dtype, n, dev = ctx.sizes, ctx.dtype, tokens.numel(), g.device
-        g = g.contiguous()
-        L = _lib.load()
-        dtable = torch.empty((v, d), dtype=dtype, device=dev)
-        nbytes = L.dg_embedding_grad_scratch_bytes(v, d, n, _DTYPES[dtype])
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        with _lib.device_ctx(dev):
-            _lib.check(L.dg_embedding_grad(g.data_ptr(), _DTYPES[dtype], tokens.data_ptr(), _WIDE[tokens.dtype], n, v, d,
-                                           ctx.scale, ctx.padding, dtable.data_ptr(), scratch.data_ptr(), nbytes,
-                                           _lib.stream_of(dev)))
-        return dtable, None, None, None
+        if torch.is_grad_enabled():    # create_graph: a second derivative would be missing this node's
+            return _table_grad_once(ctx, g)
+        return _table_grad(ctx, g)
+
+
+_table_grad_once = once_differentiable(_table_grad)
 
 
 def embedding_lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
@@ -68,20 +78,25 @@ def embedding_lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1
                            f"{tuple(table.shape)} {table.dtype}")
     if tokens.dtype not in _WIDE:
         raise RuntimeError(f"embedding_lookup: tokens must be int32 or int64, got {tokens.dtype}")
-    v = table.shape[0]
     if tokens.device != table.device:
-        if tokens.device.type != "cpu":
-            raise RuntimeError(f"embedding_lookup: tokens is on {tokens.device}, table on {table.device}")
-        if tokens.numel() and not (int(tokens.min()) >= 0 and int(tokens.max()) < v):
-            raise IndexError(f"embedding_lookup: a token is outside [0, {v})")
-        tokens = tokens.to(table.device)
+        tokens = _to_device(tokens, table)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     padding = -1
     if padding_idx is not None:
+        v = table.shape[0]
         if not -v <= padding_idx < v:
             raise IndexError(f"embedding_lookup: padding_idx {padding_idx} is outside the table's {v} rows")
         padding = padding_idx % v
     if table.requires_grad and torch.is_grad_enabled():
         return _EmbeddingLookup.apply(table, tokens, float(scale), padding)
     return _lookup(table, tokens, float(scale))
+
+
+def _to_device(tokens: torch.Tensor, table: torch.Tensor) -> torch.Tensor:
+    v = table.shape[0]
+    if tokens.device.type != "cpu":
+        raise RuntimeError(f"embedding_lookup: tokens is on {tokens.device}, table on {table.device}")
+    if tokens.numel() and not (int(tokens.min()) >= 0 and int(tokens.max()) < v):
+        raise IndexError(f"embedding_lookup: a token is outside [0, {v})")
+    return tokens.to(table.device)

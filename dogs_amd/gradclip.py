@@ -31,27 +31,25 @@ class _Table:
     """The tensors of a call as the library takes them; keeps what it points at."""
 
     def __init__(self, tensors: list, name: str, in_place: bool):
-        dev = tensors[0].device
-        ptrs, sizes, types = array("Q"), array("Q"), bytearray()
-        self.keep, self.copies = [], []
-        for t in tensors:
-            code = _DTYPES.get(t.dtype)
-            if code is None or not t.is_cuda or t.device != dev or t.layout != torch.strided:
+        self.device = tensors[0].device
+        index = tensors[0].get_device()
+        self.keep, self.copies = tensors, []
+        for k, t in enumerate(tensors):
+            if t.layout is not torch.strided or t.get_device() != index or index < 0 or t.dtype not in _DTYPES:
                 raise RuntimeError(f"{name}: gradients must be dense float32, float16 or bfloat16 tensors on one HIP "
                                    f"device, got {t.dtype} {t.layout} on {t.device}")
             if not t.is_contiguous() and not _dense(t):
-                c = t.contiguous()
+                if self.keep is tensors:
+                    self.keep = list(tensors)
+                self.keep[k] = t.contiguous()
                 if in_place:
                     if any(st == 0 and sz > 1 for st, sz in zip(t.stride(), t.shape)):
                         raise RuntimeError(f"{name}: a gradient's elements share memory: it cannot be scaled in place")
-                    self.copies.append((t, c))
-                self.keep.append(c)
-                t = c
-            ptrs.append(t.data_ptr())
-            sizes.append(t.numel())
-            types.append(code)
-        self.device, self.n = dev, len(ptrs)
-        self.ptrs, self.sizes, self.types = ptrs, sizes, array("B", types)
+                    self.copies.append((t, self.keep[k]))
+        self.n = len(tensors)
+        self.ptrs = array("Q", [t.data_ptr() for t in self.keep])
+        self.sizes = array("Q", [t.numel() for t in self.keep])
+        self.types = array("B", [_DTYPES[t.dtype] for t in self.keep])
 
     @property
     def args(self) -> tuple:
