@@ -19,32 +19,67 @@ __device__ __forceinline__ int64_t token_at(const void* t, int wide, uint32_t i)
     return wide ? ((const int64_t*)t)[i] : (int64_t)((const int32_t*)t)[i];
 }
 
-// LPR lanes (a power of two) per row, 256 / LPR rows per block; each lane moves 16 bytes at a time
+// A lane's 16 bytes of a row
+template <typename T> struct Cols {
+    typedef typename Vec<T>::type V;
+    static constexpr int W = Vec<T>::W;
+    uint32_t c0;     // first column of this lane
+    int nc;          // its columns: W, 0 past the row, or the whole row where that is shorter than W
+    __device__ __forceinline__ V load(const T* row) const {
+        V x = {};
+        if (nc == W) x = *reinterpret_cast<const V*>(row + c0);
+        else
+            for (int j = 0; j < nc; j++) x[j] = row[j];
+        return x;
+    }
+    __device__ __forceinline__ void store(T* row, V x) const {
+        if (nc == W) *reinterpret_cast<V*>(row + c0) = x;
+        else
+            for (int j = 0; j < nc; j++) row[j] = x[j];
+    }
+    __device__ __forceinline__ void store(T* row, const float (&acc)[W], float scale) const {
+        V x;
+#pragma unroll
+        for (int j = 0; j < W; j++) x[j] = (T)(acc[j] * scale);
+        store(row, x);
+    }
+};
+
+// The last lane of a row whose width is no multiple of W takes the row's last W columns: some are the lane's before it too, and
+// both compute and store the same bits.  (Its own few columns one by one: a row of 1023 fp16 took 2.7 times as long
+// as one of 1024.)
 template <typename T>
-__global__ void __launch_bounds__(EB_THREADS) k_lookup(LookupArgs a, int lpr) {
+__device__ __forceinline__ Cols<T> cols_of(uint32_t slab, int lpr, uint32_t l, uint32_t D) {
+    constexpr uint32_t W = Vec<T>::W;
+    const uint64_t c0 = ((uint64_t)slab * lpr + l) * W;
+    if (D < W) return {0u, c0 ? 0 : (int)D};
+    if (c0 >= D) return {0u, 0};
+    return {c0 + W <= D ? (uint32_t)c0 : D - W, (int)W};
+}
+
+// lpr lanes (a power of two) per row, 256 / lpr rows per block
+template <typename T>
+__global__ void __launch_bounds__(EB_THREADS) k_lookup(LookupArgs a, int lpr, uint32_t slabs) {
     typedef typename Vec<T>::type V;
     constexpr int W = Vec<T>::W;
     const uint32_t l = threadIdx.x & (lpr - 1), per = EB_THREADS / lpr;
     for (uint64_t row = (uint64_t)blockIdx.x * per + threadIdx.x / lpr; row < a.n; row += (uint64_t)gridDim.x * per) {
         const int64_t tok = token_at(a.tokens, a.wide, (uint32_t)row);
+        const bool bad = tok < 0 || (uint64_t)tok >= a.V;
         T* out = (T*)a.out + row * a.D;
-        if (tok < 0 || (uint64_t)tok >= a.V) {
-            for (uint32_t c = l; c < a.D; c += lpr) out[c] = (T)__builtin_nanf("");
-            continue;
-        }
-        const T* in = (const T*)a.table + tok * a.row_stride;
+        const T* in = (const T*)a.table + (bad ? 0 : tok) * a.row_stride;
         if (a.col_stride != 1) {
-            for (uint32_t c = l; c < a.D; c += lpr) out[c] = (T)((float)in[c * a.col_stride] * a.scale);
+            for (uint32_t c = l; c < a.D; c += lpr) out[c] = (T)(bad ? __builtin_nanf("") : (float)in[(int64_t)c * a.col_stride] * a.scale);
             continue;
         }
-        const uint32_t nv = a.D / W;
-        for (uint32_t c = l; c < nv; c += lpr) {
-            V x = *reinterpret_cast<const V*>(in + (uint64_t)c * W);
+        for (uint32_t slab = 0; slab < slabs; slab++) {
+            const Cols<T> c = cols_of<T>(slab, lpr, l, a.D);
+            V x = {};
+            if (!bad) x = c.load(in);
 #pragma unroll
-            for (int j = 0; j < W; j++) x[j] = (T)((float)x[j] * a.scale);
-            *reinterpret_cast<V*>(out + (uint64_t)c * W) = x;
+            for (int j = 0; j < W; j++) x[j] = (T)(bad ? __builtin_nanf("") : (float)x[j] * a.scale);
+            c.store(out, x);
         }
-        for (uint32_t c = nv * W + l; c < a.D; c += lpr) out[c] = (T)((float)in[c] * a.scale);
     }
 }
 
@@ -96,47 +131,18 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s_w) {
 // a row whose entries lie within one part is stored from there.  Sums of runs that cross parts meet in LDS, in order, and
 // those that cross the block's ends go to the partials of the block: `head` for the run that began before it,
 // `tail` for the one that begins in it and goes on.  So a token that makes up half the batch costs no more than others.
-template <typename T> struct Cols {
-    typedef typename Vec<T>::type V;
-    static constexpr int W = Vec<T>::W;
-    uint32_t c0;     // first column of this lane
-    int nc;          // how many of its W columns exist
-    __device__ __forceinline__ V load(const T* row) const {
-        if (nc == W) return *reinterpret_cast<const V*>(row + c0);
-        V x = {};
-#pragma unroll
-        for (int j = 0; j < W; j++)
-            if (j < nc) x[j] = row[c0 + j];
-        return x;
-    }
-    __device__ __forceinline__ void store(T* row, const float (&acc)[W], float scale) const {
-        V x;
-#pragma unroll
-        for (int j = 0; j < W; j++) x[j] = (T)(acc[j] * scale);
-        if (nc == W) {
-            *reinterpret_cast<V*>(row + c0) = x;
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < W; j++)
-            if (j < nc) row[c0 + j] = x[j];
-    }
-    __device__ __forceinline__ void zero(T* row) const {
-        const float z[W] = {};
-        store(row, z, 0.0f);
-    }
+struct Pairs {       // a list in LDS as two arrays
+    const uint32_t *k, *p;
+    __device__ __forceinline__ uint32_t key(uint32_t j) const { return k[j]; }
+    __device__ __forceinline__ uint32_t pos(uint32_t j) const { return p[j]; }
 };
-
-template <typename T>
-__device__ __forceinline__ Cols<T> cols_of(uint32_t slab, int lpr, uint32_t l, uint32_t D) {
-    const uint64_t c0 = ((uint64_t)slab * lpr + l) * Vec<T>::W;
-    const int64_t left = (int64_t)D - (int64_t)c0;
-    return {(uint32_t)c0, left >= Vec<T>::W ? Vec<T>::W : left > 0 ? (int)left : 0};
-}
-
-struct Stretch {
-    const uint32_t* key;     // LDS, ascending
-    const uint32_t* pos;     // LDS
+struct Packed {      // as key << 16 | position
+    const uint32_t* e;
+    __device__ __forceinline__ uint32_t key(uint32_t j) const { return e[j] >> 16; }
+    __device__ __forceinline__ uint32_t pos(uint32_t j) const { return e[j] & 0xffffu; }
+};
+template <typename L> struct Stretch {
+    L e;                     // ascending keys
     uint32_t n;
     bool open_front, open_back;   // the first / last run goes on outside
     uint32_t row0;           // key k is row row0 + k of the table
@@ -146,8 +152,8 @@ struct Stretch {
 constexpr int WALK = 8;
 
 // THREADS threads; s_part: LDS of THREADS * 2 * W floats
-template <typename T, int THREADS>
-__device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stretch& s, const Cols<T>& c, int lpr,
+template <typename T, int THREADS, typename L>
+__device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stretch<L>& s, const Cols<T>& c, int lpr,
                                             float* __restrict__ s_part) {
     typedef typename Vec<T>::type V;
     constexpr int W = Vec<T>::W;
@@ -157,10 +163,10 @@ __device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stret
     T* table = (T*)a.dtable;
     float* mine = s_part + threadIdx.x * (2 * W);   // this lane's columns of the group's head, then of its tail
     if (lo < hi) {
-        const bool front = lo ? s.key[lo - 1] == s.key[lo] : s.open_front;
-        const bool back = hi < s.n ? s.key[hi] == s.key[hi - 1] : s.open_back;
+        const bool front = lo ? s.e.key(lo - 1) == s.e.key(lo) : s.open_front;
+        const bool back = hi < s.n ? s.e.key(hi) == s.e.key(hi - 1) : s.open_back;
         float acc[W] = {};
-        uint32_t cur = s.key[lo];
+        uint32_t cur = s.e.key(lo);
         bool first = true;
         auto flush = [&](bool last) {
             if (first && front) {
@@ -179,8 +185,8 @@ __device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stret
 #pragma unroll
             for (int u = 0; u < WALK; u++) {
                 const uint32_t j = j0 + u < hi ? j0 + u : hi - 1;
-                k[u] = s.key[j];
-                x[u] = c.load(grad + (uint64_t)s.pos[j] * a.D);
+                k[u] = s.e.key(j);
+                x[u] = c.load(grad + (uint64_t)s.e.pos(j) * a.D);
             }
 #pragma unroll
             for (int u = 0; u < WALK; u++) {
@@ -203,7 +209,7 @@ __device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stret
     // the group whose tail begins a run joins it with the heads after it; group 0 also joins the run that was open in front
     const uint32_t lane_off = (threadIdx.x - g * lpr) * (2 * W);
     auto join = [&](float (&acc)[W], uint32_t k, uint32_t h) {   // heads of parts h, h + 1, ... while they hold key k
-        for (; h < groups && h * part < s.n && s.key[h * part] == k; h++) {
+        for (; h < groups && h * part < s.n && s.e.key(h * part) == k; h++) {
             const float* o = s_part + (uint64_t)h * lpr * (2 * W) + lane_off;
 #pragma unroll
             for (int j = 0; j < W; j++) acc[j] += o[j];
@@ -218,18 +224,18 @@ __device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stret
         float acc[W];
 #pragma unroll
         for (int j = 0; j < W; j++) acc[j] = mine[j];
-        join(acc, s.key[0], 1);
+        join(acc, s.e.key(0), 1);
         put(s.head, acc);
     }
-    const uint32_t k = s.key[hi - 1];
-    const bool begins = lo ? s.key[lo - 1] != k : !(s.open_front && s.key[0] == k);
-    const bool goes_on = hi < s.n ? s.key[hi] == k : s.open_back;
+    const uint32_t k = s.e.key(hi - 1);
+    const bool begins = lo ? s.e.key(lo - 1) != k : !(s.open_front && s.e.key(0) == k);
+    const bool goes_on = hi < s.n ? s.e.key(hi) == k : s.open_back;
     if (begins && goes_on) {
         float acc[W];
 #pragma unroll
         for (int j = 0; j < W; j++) acc[j] = mine[W + j];
         join(acc, k, g + 1);
-        if (s.open_back && s.key[s.n - 1] == k) put(s.tail, acc);
+        if (s.open_back && s.e.key(s.n - 1) == k) put(s.tail, acc);
         else c.store(table + (uint64_t)(s.row0 + k) * a.D, acc, a.scale);
     }
 }
@@ -238,10 +244,10 @@ __device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stret
 //
 // A block owns `rows` (a power of two, up to 256) rows of the table and one slab of columns.  It looks through all tokens,
 // each wave through a contiguous part of them, ranks those of its rows (stable counting sort by row, in LDS), and sums.
-template <typename T, int NW>
+// The list is 64 IT NW entries long at most; LDS and the tokens that a lane looks at go with it.
+template <typename T, int NW, int IT>
 __global__ void __launch_bounds__(NW * 64) k_grad_small(LookupGradArgs a, int lpr, uint32_t rows, int row_bits, uint32_t slabs) {
-    constexpr int IT = 16, CAP = NW * 64 * IT;
-    __shared__ uint32_t s_key[CAP], s_pos[CAP];
+    __shared__ uint32_t s_list[NW * 64 * IT];
     __shared__ uint32_t s_hist[NW][256];
     __shared__ uint32_t s_w[NW];
     __shared__ float s_part[NW * 64 * 2 * Vec<T>::W];
@@ -290,17 +296,16 @@ __global__ void __launch_bounds__(NW * 64) k_grad_small(LookupGradArgs a, int lp
     for (int r = 0; r < IT; r++) {
         if (code[r] == ~0u) continue;
         const uint32_t lr = code[r] >> 16, o = s_hist[w][lr] + (code[r] & 0xffffu);
-        s_key[o] = lr;
-        s_pos[o] = base + 64 * r;
+        s_list[o] = lr << 16 | (base + 64 * r);
     }
     __syncthreads();
     const Cols<T> c = cols_of<T>(slab, lpr, t & (lpr - 1), a.D);
     // rows without a token: the last wave's start of row r, advanced past its tokens, is where row r + 1 begins
     for (uint32_t r = t / lpr; r < nrows; r += NW * 64 / lpr) {
         const uint32_t end = r + 1 < 256 ? s_hist[0][r + 1] : total;
-        if (s_hist[0][r] == end) c.zero((T*)a.dtable + (uint64_t)(v0 + r) * a.D);
+        if (s_hist[0][r] == end) c.store((T*)a.dtable + (uint64_t)(v0 + r) * a.D, typename Vec<T>::type{});
     }
-    const Stretch s = {s_key, s_pos, total, false, false, v0, nullptr, nullptr};
+    const Stretch<Packed> s = {{s_list}, total, false, false, v0, nullptr, nullptr};
     sum_stretch<T, NW * 64>(a, s, c, lpr, s_part);
 }
 
@@ -459,7 +464,7 @@ __global__ void __launch_bounds__(EB_THREADS) k_grad_sums(LookupGradArgs a, SumP
         if (s_key[n - 1] == a.V) n = lower_bound(s_key, n, a.V);   // entries that add to no row are last
         if (!n) return;
         float* part = p.partial + (uint64_t)c * 2 * a.D;
-        const Stretch s = {s_key, s_pos, n, before == s_key[0], n == e1 - e0 && after == s_key[n - 1], 0, part, part + a.D};
+        const Stretch<Pairs> s = {{s_key, s_pos}, n, before == s_key[0], n == e1 - e0 && after == s_key[n - 1], 0, part, part + a.D};
         sum_stretch<T, EB_THREADS>(a, s, cols_of<T>(slab, p.lpr, l, a.D), p.lpr, s_part);
         return;
     }
@@ -478,7 +483,7 @@ __global__ void __launch_bounds__(EB_THREADS) k_grad_sums(LookupGradArgs a, SumP
     for (uint32_t r = threadIdx.x / p.lpr; r < p.zero_rows; r += groups)
         if (s_key[r])
             for (uint32_t slab = 0; slab < p.slabs; slab++)
-                cols_of<T>(slab, p.lpr, l, a.D).zero((T*)a.dtable + (v0 + r) * a.D);
+                cols_of<T>(slab, p.lpr, l, a.D).store((T*)a.dtable + (v0 + r) * a.D, typename Vec<T>::type{});
 }
 
 // The runs that cross stretches: the block of the stretch where one begins adds the tail there and the heads after it, a
@@ -537,18 +542,6 @@ int key_bits(uint32_t V) {
 
 }  // namespace
 
-void launch_embedding_lookup(const LookupArgs& a, int dtype, hipStream_t s) {
-    const uint32_t W = 16 / elem_bytes(dtype), chunks = (a.D + W - 1) / W;
-    int lpr = 1;
-    while (lpr < EB_THREADS && (uint32_t)lpr < chunks) lpr <<= 1;
-    const uint32_t rows = EB_THREADS / lpr;
-    uint32_t blocks = (uint32_t)(((uint64_t)a.n + rows - 1) / rows);
-    if (blocks > EB_MAX_BLOCKS) blocks = EB_MAX_BLOCKS;
-    if (dtype == 0) k_lookup<float><<<blocks, EB_THREADS, 0, s>>>(a, lpr);
-    else if (dtype == 1) k_lookup<_Float16><<<blocks, EB_THREADS, 0, s>>>(a, lpr);
-    else k_lookup<__bf16><<<blocks, EB_THREADS, 0, s>>>(a, lpr);
-}
-
 namespace {
 
 // lanes of a row's slab: as many 16-byte pieces as the row has, up to a wave
@@ -600,7 +593,9 @@ void grad_small(const LookupGradArgs& a, int dtype, hipStream_t s) {
     int bits = 0;
     while (rows < 256 && (uint64_t)((a.V + rows - 1) / rows) * slabs > 1024) { rows <<= 1; bits++; }
     const uint64_t blocks = (uint64_t)((a.V + rows - 1) / rows) * slabs;
-    k_grad_small<T, 4><<<(uint32_t)blocks, 256, 0, s>>>(a, lpr, rows, bits, slabs);
+    if (a.n <= 1024) k_grad_small<T, 4, 4><<<(uint32_t)blocks, 256, 0, s>>>(a, lpr, rows, bits, slabs);
+    else if (a.n <= 4096) k_grad_small<T, 4, 16><<<(uint32_t)blocks, 256, 0, s>>>(a, lpr, rows, bits, slabs);
+    else k_grad_small<T, 16, 16><<<(uint32_t)blocks, 1024, 0, s>>>(a, lpr, rows, bits, slabs);
 }
 
 template <typename T>
@@ -611,6 +606,16 @@ void grad_sums(const LookupGradArgs& a, const SumPlan& p, hipStream_t s) {
 }
 
 }  // namespace
+
+void launch_embedding_lookup(const LookupArgs& a, int dtype, hipStream_t s) {
+    const int lpr = lanes_per_row(a.D, dtype, EB_THREADS);
+    const uint32_t rows = EB_THREADS / lpr, slabs = slabs_of(a.D, dtype, lpr);
+    uint32_t blocks = (uint32_t)(((uint64_t)a.n + rows - 1) / rows);
+    if (blocks > EB_MAX_BLOCKS) blocks = EB_MAX_BLOCKS;
+    if (dtype == 0) k_lookup<float><<<blocks, EB_THREADS, 0, s>>>(a, lpr, slabs);
+    else if (dtype == 1) k_lookup<_Float16><<<blocks, EB_THREADS, 0, s>>>(a, lpr, slabs);
+    else k_lookup<__bf16><<<blocks, EB_THREADS, 0, s>>>(a, lpr, slabs);
+}
 
 size_t embedding_grad_scratch_bytes(uint32_t V, uint32_t D, uint32_t n, int dtype) {
     if (n <= SMALL_N) return 0;

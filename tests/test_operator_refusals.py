@@ -41,10 +41,10 @@ def test_embedding_entry_refusals(lib):
 
     def grad(g=16, dtype=0, v=4, d=4, tokens=16, n=2, out=16, scratch=256, nbytes=1 << 20):
         return lib.dg_embedding_grad(g, dtype, tokens, 1, n, v, d, 1.0, -1, out, scratch, nbytes, None)
-    need = lib.dg_embedding_grad_scratch_bytes(4, 4, 10000, 0)
+    need = lib.dg_embedding_grad_scratch_bytes(4, 4, 20000, 0)
     assert need > 0
     for kw in ({"dtype": 3}, {"v": 1 << 31}, {"n": 1 << 31}, {"d": 1 << 23}, {"g": None}, {"tokens": None}, {"out": None},
-               {"n": 10000, "scratch": None}, {"n": 10000, "nbytes": need - 1}):
+               {"n": 20000, "scratch": None}, {"n": 20000, "nbytes": need - 1}):
         assert grad(**kw) != 0, kw
     assert grad(v=0) == 0 and grad(d=0) == 0
     assert lib.dg_embedding_grad_scratch_bytes(1 << 31, 4, 2, 0) == 0
