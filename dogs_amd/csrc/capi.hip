@@ -1298,7 +1298,7 @@ static int grad_norm_impl(int n_tensors, const void* const* tensors, const uint6
     double* partial = (double*)((char*)scratch + 256);
     uint32_t b = 0;
     for (const gs::GradTable& t : tables) {
-        gs::launch_grad_partials(t, ord, partial + b, s);
+        gs::launch_grad_partials(t, ord, coef != nullptr, partial + b, s);
         b += t.start[t.count];
     }
     gs::launch_grad_norm_final(partial, blocks, ord, max_norm, norm, coef, s);

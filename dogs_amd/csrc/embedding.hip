@@ -13,28 +13,36 @@ namespace gs {
 namespace {
 
 constexpr int EB_THREADS = 256;
+constexpr uint64_t PAST_BYTES = 32ull << 20;   // the L2 caches together
 constexpr uint32_t EB_MAX_BLOCKS = 1u << 20;   // then they stride: a grid holds fewer than 2^32 threads
 
 __device__ __forceinline__ int64_t token_at(const void* t, int wide, uint32_t i) {
     return wide ? ((const int64_t*)t)[i] : (int64_t)((const int32_t*)t)[i];
 }
 
-// A lane's 16 bytes of a row
-template <typename T> struct Cols {
+// A lane's 16 bytes of a row.  PAST: by the caches, where what is touched once is larger than they are -- 65536 x 2048 bf16
+// in 131072 rows: the sums 139 us instead of 190, the lookup 72 instead of 84; smaller results stay in the caches for the
+// kernel that reads them.
+template <typename T, bool PAST> struct Cols {
     typedef typename Vec<T>::type V;
     static constexpr int W = Vec<T>::W;
     uint32_t c0;     // first column of this lane
     int nc;          // its columns: W, 0 past the row, or the whole row where that is shorter than W
+    template <bool ONCE>
     __device__ __forceinline__ V load(const T* row) const {
         V x = {};
-        if (nc == W) x = *reinterpret_cast<const V*>(row + c0);
+        const V* q = reinterpret_cast<const V*>(row + c0);
+        if (nc == W) x = PAST && ONCE ? __builtin_nontemporal_load(q) : *q;
         else
             for (int j = 0; j < nc; j++) x[j] = row[j];
         return x;
     }
     __device__ __forceinline__ void store(T* row, V x) const {
-        if (nc == W) *reinterpret_cast<V*>(row + c0) = x;
-        else
+        V* q = reinterpret_cast<V*>(row + c0);
+        if (nc == W) {
+            if (PAST) __builtin_nontemporal_store(x, q);
+            else *q = x;
+        } else
             for (int j = 0; j < nc; j++) row[j] = x[j];
     }
     __device__ __forceinline__ void store(T* row, const float (&acc)[W], float scale) const {
@@ -48,8 +56,8 @@ template <typename T> struct Cols {
 // The last lane of a row whose width is no multiple of W takes the row's last W columns: some are the lane's before it too, and
 // both compute and store the same bits.  (Its own few columns one by one: a row of 1023 fp16 took 2.7 times as long
 // as one of 1024.)
-template <typename T>
-__device__ __forceinline__ Cols<T> cols_of(uint32_t slab, int lpr, uint32_t l, uint32_t D) {
+template <typename T, bool PAST>
+__device__ __forceinline__ Cols<T, PAST> cols_of(uint32_t slab, int lpr, uint32_t l, uint32_t D) {
     constexpr uint32_t W = Vec<T>::W;
     const uint64_t c0 = ((uint64_t)slab * lpr + l) * W;
     if (D < W) return {0u, c0 ? 0 : (int)D};
@@ -57,28 +65,34 @@ __device__ __forceinline__ Cols<T> cols_of(uint32_t slab, int lpr, uint32_t l, u
     return {c0 + W <= D ? (uint32_t)c0 : D - W, (int)W};
 }
 
-// lpr lanes (a power of two) per row, 256 / lpr rows per block
-template <typename T>
-__global__ void __launch_bounds__(EB_THREADS) k_lookup(LookupArgs a, int lpr, uint32_t slabs) {
+// lpr lanes (a power of two, up to a wave) per row, 256 / lpr rows per block, LOOK slabs of a row in flight: one where there
+// are few rows (a block per slab), four for a large result
+template <typename T, int LOOK, bool PAST>
+__global__ void __launch_bounds__(EB_THREADS) k_lookup(LookupArgs a, int lpr) {
     typedef typename Vec<T>::type V;
     constexpr int W = Vec<T>::W;
     const uint32_t l = threadIdx.x & (lpr - 1), per = EB_THREADS / lpr;
+    Cols<T, PAST> c[LOOK];
+#pragma unroll
+    for (int u = 0; u < LOOK; u++) c[u] = cols_of<T, PAST>(blockIdx.y * LOOK + u, lpr, l, a.D);
     for (uint64_t row = (uint64_t)blockIdx.x * per + threadIdx.x / lpr; row < a.n; row += (uint64_t)gridDim.x * per) {
         const int64_t tok = token_at(a.tokens, a.wide, (uint32_t)row);
         const bool bad = tok < 0 || (uint64_t)tok >= a.V;
         T* out = (T*)a.out + row * a.D;
         const T* in = (const T*)a.table + (bad ? 0 : tok) * a.row_stride;
         if (a.col_stride != 1) {
-            for (uint32_t c = l; c < a.D; c += lpr) out[c] = (T)(bad ? __builtin_nanf("") : (float)in[(int64_t)c * a.col_stride] * a.scale);
+            for (uint32_t k = blockIdx.y * lpr + l; k < a.D; k += gridDim.y * lpr)
+                out[k] = (T)(bad ? __builtin_nanf("") : (float)in[(int64_t)k * a.col_stride] * a.scale);
             continue;
         }
-        for (uint32_t slab = 0; slab < slabs; slab++) {
-            const Cols<T> c = cols_of<T>(slab, lpr, l, a.D);
-            V x = {};
-            if (!bad) x = c.load(in);
+        V x[LOOK];
 #pragma unroll
-            for (int j = 0; j < W; j++) x[j] = (T)(bad ? __builtin_nanf("") : (float)x[j] * a.scale);
-            c.store(out, x);
+        for (int u = 0; u < LOOK; u++) x[u] = bad ? V{} : c[u].template load<false>(in);
+#pragma unroll
+        for (int u = 0; u < LOOK; u++) {
+#pragma unroll
+            for (int j = 0; j < W; j++) x[u][j] = (T)(bad ? __builtin_nanf("") : (float)x[u][j] * a.scale);
+            c[u].store(out, x[u]);
         }
     }
 }
@@ -152,8 +166,8 @@ template <typename L> struct Stretch {
 constexpr int WALK = 8;
 
 // THREADS threads; s_part: LDS of THREADS * 2 * W floats
-template <typename T, int THREADS, typename L>
-__device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stretch<L>& s, const Cols<T>& c, int lpr,
+template <typename T, bool PAST, int THREADS, typename L>
+__device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stretch<L>& s, const Cols<T, PAST>& c, int lpr,
                                             float* __restrict__ s_part) {
     typedef typename Vec<T>::type V;
     constexpr int W = Vec<T>::W;
@@ -186,7 +200,7 @@ __device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stret
             for (int u = 0; u < WALK; u++) {
                 const uint32_t j = j0 + u < hi ? j0 + u : hi - 1;
                 k[u] = s.e.key(j);
-                x[u] = c.load(grad + (uint64_t)s.e.pos(j) * a.D);
+                x[u] = c.template load<true>(grad + (uint64_t)s.e.pos(j) * a.D);
             }
 #pragma unroll
             for (int u = 0; u < WALK; u++) {
@@ -245,7 +259,7 @@ __device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stret
 // A block owns `rows` (a power of two, up to 256) rows of the table and one slab of columns.  It looks through all tokens,
 // each wave through a contiguous part of them, ranks those of its rows (stable counting sort by row, in LDS), and sums.
 // The list is 64 IT NW entries long at most; LDS and the tokens that a lane looks at go with it.
-template <typename T, int NW, int IT>
+template <typename T, bool PAST, int NW, int IT>
 __global__ void __launch_bounds__(NW * 64) k_grad_small(LookupGradArgs a, int lpr, uint32_t rows, int row_bits, uint32_t slabs) {
     __shared__ uint32_t s_list[NW * 64 * IT];
     __shared__ uint32_t s_hist[NW][256];
@@ -299,14 +313,14 @@ __global__ void __launch_bounds__(NW * 64) k_grad_small(LookupGradArgs a, int lp
         s_list[o] = lr << 16 | (base + 64 * r);
     }
     __syncthreads();
-    const Cols<T> c = cols_of<T>(slab, lpr, t & (lpr - 1), a.D);
+    const Cols<T, PAST> c = cols_of<T, PAST>(slab, lpr, t & (lpr - 1), a.D);
     // rows without a token: the last wave's start of row r, advanced past its tokens, is where row r + 1 begins
     for (uint32_t r = t / lpr; r < nrows; r += NW * 64 / lpr) {
         const uint32_t end = r + 1 < 256 ? s_hist[0][r + 1] : total;
         if (s_hist[0][r] == end) c.store((T*)a.dtable + (uint64_t)(v0 + r) * a.D, typename Vec<T>::type{});
     }
     const Stretch<Packed> s = {{s_list}, total, false, false, v0, nullptr, nullptr};
-    sum_stretch<T, NW * 64>(a, s, c, lpr, s_part);
+    sum_stretch<T, PAST, NW * 64>(a, s, c, lpr, s_part);
 }
 
 // ---- many tokens: sort them, sum stretches of the sorted list, join what crosses stretches
@@ -445,7 +459,7 @@ struct SumPlan {
 constexpr uint32_t MAX_ENTRIES = 2048;
 
 // blocks [0, stretches * slabs): the sums; the rest: zeros in the rows that no token names
-template <typename T>
+template <typename T, bool PAST>
 __global__ void __launch_bounds__(EB_THREADS) k_grad_sums(LookupGradArgs a, SumPlan p) {
     __shared__ uint32_t s_key[MAX_ENTRIES], s_pos[MAX_ENTRIES];
     __shared__ float s_part[EB_THREADS * 2 * Vec<T>::W];
@@ -465,7 +479,7 @@ __global__ void __launch_bounds__(EB_THREADS) k_grad_sums(LookupGradArgs a, SumP
         if (!n) return;
         float* part = p.partial + (uint64_t)c * 2 * a.D;
         const Stretch<Pairs> s = {{s_key, s_pos}, n, before == s_key[0], n == e1 - e0 && after == s_key[n - 1], 0, part, part + a.D};
-        sum_stretch<T, EB_THREADS>(a, s, cols_of<T>(slab, p.lpr, l, a.D), p.lpr, s_part);
+        sum_stretch<T, PAST, EB_THREADS>(a, s, cols_of<T, PAST>(slab, p.lpr, l, a.D), p.lpr, s_part);
         return;
     }
     const uint64_t v0 = (blockIdx.x - sums) * p.zero_rows;
@@ -483,7 +497,7 @@ __global__ void __launch_bounds__(EB_THREADS) k_grad_sums(LookupGradArgs a, SumP
     for (uint32_t r = threadIdx.x / p.lpr; r < p.zero_rows; r += groups)
         if (s_key[r])
             for (uint32_t slab = 0; slab < p.slabs; slab++)
-                cols_of<T>(slab, p.lpr, l, a.D).store((T*)a.dtable + (v0 + r) * a.D, typename Vec<T>::type{});
+                cols_of<T, PAST>(slab, p.lpr, l, a.D).store((T*)a.dtable + (v0 + r) * a.D, typename Vec<T>::type{});
 }
 
 // The runs that cross stretches: the block of the stretch where one begins adds the tail there and the heads after it, a
@@ -545,10 +559,10 @@ int key_bits(uint32_t V) {
 namespace {
 
 // lanes of a row's slab: as many 16-byte pieces as the row has, up to a wave
-int lanes_per_row(uint32_t D, int dtype, int most) {
+int lanes_per_row(uint32_t D, int dtype) {
     const uint32_t W = 16 / elem_bytes(dtype), pieces = (D + W - 1) / W;
     int lpr = 1;
-    while (lpr < most && (uint32_t)lpr < pieces) lpr <<= 1;
+    while (lpr < 64 && (uint32_t)lpr < pieces) lpr <<= 1;
     return lpr;
 }
 uint32_t slabs_of(uint32_t D, int dtype, int lpr) {
@@ -556,11 +570,14 @@ uint32_t slabs_of(uint32_t D, int dtype, int lpr) {
     return (D + per - 1) / per;
 }
 
-constexpr uint32_t SMALL_N = 4096;   // as many tokens as the one-launch kernel holds
+// As many tokens as the one-launch kernel holds.  At 8000 tokens it and the sort with what follows take about as long (64 fp32
+// over 2000 rows 17 us; 1023 fp16 over 50021 rows 48 us and 50), but it is one launch, not eight; a block of 16 waves
+// for 16384 tokens fills a CU alone and was slower (62 us at 8191).
+constexpr uint32_t SMALL_N = 8192;
 
 SumPlan plan_of(const LookupGradArgs& a, int dtype) {
     SumPlan p = {};
-    p.lpr = lanes_per_row(a.D, dtype, 64);
+    p.lpr = lanes_per_row(a.D, dtype);
     p.slabs = slabs_of(a.D, dtype, p.lpr);
     const uint32_t groups = EB_THREADS / p.lpr;
     p.entries = 32 * groups < MAX_ENTRIES ? 32 * groups : MAX_ENTRIES;
@@ -585,36 +602,46 @@ GradScratch scratch_of(const LookupGradArgs& a, const SumPlan& p) {
     return s;
 }
 
-template <typename T>
+bool past_caches(const LookupGradArgs& a, int dtype) {
+    return ((uint64_t)a.n + a.V) * a.D * elem_bytes(dtype) >= 2 * PAST_BYTES;
+}
+
+template <typename T, bool PAST>
 void grad_small(const LookupGradArgs& a, int dtype, hipStream_t s) {
-    const int lpr = lanes_per_row(a.D, dtype, 64);
+    const int lpr = lanes_per_row(a.D, dtype);
     const uint32_t slabs = slabs_of(a.D, dtype, lpr);
     uint32_t rows = 1;
     int bits = 0;
     while (rows < 256 && (uint64_t)((a.V + rows - 1) / rows) * slabs > 1024) { rows <<= 1; bits++; }
     const uint64_t blocks = (uint64_t)((a.V + rows - 1) / rows) * slabs;
-    if (a.n <= 1024) k_grad_small<T, 4, 4><<<(uint32_t)blocks, 256, 0, s>>>(a, lpr, rows, bits, slabs);
-    else if (a.n <= 4096) k_grad_small<T, 4, 16><<<(uint32_t)blocks, 256, 0, s>>>(a, lpr, rows, bits, slabs);
-    else k_grad_small<T, 16, 16><<<(uint32_t)blocks, 1024, 0, s>>>(a, lpr, rows, bits, slabs);
+    if (a.n <= 1024) k_grad_small<T, PAST, 4, 4><<<(uint32_t)blocks, 256, 0, s>>>(a, lpr, rows, bits, slabs);
+    else if (a.n <= 4096) k_grad_small<T, PAST, 4, 16><<<(uint32_t)blocks, 256, 0, s>>>(a, lpr, rows, bits, slabs);
+    else k_grad_small<T, PAST, 8, 16><<<(uint32_t)blocks, 512, 0, s>>>(a, lpr, rows, bits, slabs);
 }
 
-template <typename T>
+template <typename T, bool PAST>
 void grad_sums(const LookupGradArgs& a, const SumPlan& p, hipStream_t s) {
     const uint64_t blocks = (uint64_t)p.stretches * p.slabs + ((uint64_t)a.V + p.zero_rows - 1) / p.zero_rows;
-    k_grad_sums<T><<<(uint32_t)blocks, EB_THREADS, 0, s>>>(a, p);
+    k_grad_sums<T, PAST><<<(uint32_t)blocks, EB_THREADS, 0, s>>>(a, p);
     if (p.stretches > 1) k_grad_join<T><<<dim3(p.stretches - 1, (a.D + 255) / 256), EB_THREADS, 0, s>>>(a, p);
 }
 
 }  // namespace
 
 void launch_embedding_lookup(const LookupArgs& a, int dtype, hipStream_t s) {
-    const int lpr = lanes_per_row(a.D, dtype, EB_THREADS);
+    const int lpr = lanes_per_row(a.D, dtype);
     const uint32_t rows = EB_THREADS / lpr, slabs = slabs_of(a.D, dtype, lpr);
-    uint32_t blocks = (uint32_t)(((uint64_t)a.n + rows - 1) / rows);
-    if (blocks > EB_MAX_BLOCKS) blocks = EB_MAX_BLOCKS;
-    if (dtype == 0) k_lookup<float><<<blocks, EB_THREADS, 0, s>>>(a, lpr, slabs);
-    else if (dtype == 1) k_lookup<_Float16><<<blocks, EB_THREADS, 0, s>>>(a, lpr, slabs);
-    else k_lookup<__bf16><<<blocks, EB_THREADS, 0, s>>>(a, lpr, slabs);
+    const bool large = (uint64_t)a.n * a.D * elem_bytes(dtype) >= PAST_BYTES;
+    const uint64_t blocks = ((uint64_t)a.n + rows - 1) / rows;
+    const dim3 grid((uint32_t)(blocks < EB_MAX_BLOCKS ? blocks : EB_MAX_BLOCKS), large ? (slabs + 3) / 4 : slabs);
+    auto go = [&](auto t) {
+        typedef decltype(t) T;
+        if (large) k_lookup<T, 4, true><<<grid, EB_THREADS, 0, s>>>(a, lpr);
+        else k_lookup<T, 1, false><<<grid, EB_THREADS, 0, s>>>(a, lpr);
+    };
+    if (dtype == 0) go(float());
+    else if (dtype == 1) go(_Float16());
+    else go(__bf16());
 }
 
 size_t embedding_grad_scratch_bytes(uint32_t V, uint32_t D, uint32_t n, int dtype) {
@@ -626,9 +653,13 @@ size_t embedding_grad_scratch_bytes(uint32_t V, uint32_t D, uint32_t n, int dtyp
 
 void launch_embedding_grad(const LookupGradArgs& a, int dtype, void* scratch, hipStream_t s) {
     if (a.n <= SMALL_N) {
-        if (dtype == 0) grad_small<float>(a, dtype, s);
-        else if (dtype == 1) grad_small<_Float16>(a, dtype, s);
-        else grad_small<__bf16>(a, dtype, s);
+        auto go = [&](auto t) {
+            if (past_caches(a, dtype)) grad_small<decltype(t), true>(a, dtype, s);
+            else grad_small<decltype(t), false>(a, dtype, s);
+        };
+        if (dtype == 0) go(float());
+        else if (dtype == 1) go(_Float16());
+        else go(__bf16());
         return;
     }
     SumPlan p = plan_of(a, dtype);
@@ -658,9 +689,13 @@ void launch_embedding_grad(const LookupGradArgs& a, int dtype, void* scratch, hi
     p.keys = k[in];
     p.pos = v[in];
     p.partial = (float*)(b + o.partial);
-    if (dtype == 0) grad_sums<float>(a, p, s);
-    else if (dtype == 1) grad_sums<_Float16>(a, p, s);
-    else grad_sums<__bf16>(a, p, s);
+    auto go = [&](auto t) {
+        if (past_caches(a, dtype)) grad_sums<decltype(t), true>(a, p, s);
+        else grad_sums<decltype(t), false>(a, p, s);
+    };
+    if (dtype == 0) go(float());
+    else if (dtype == 1) go(_Float16());
+    else go(__bf16());
 }
 
 }  // namespace gs

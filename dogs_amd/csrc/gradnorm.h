@@ -25,8 +25,9 @@ struct GradTable {
 // the chunk size at which the tensors take at most GN_MAX_BLOCKS (+ one per tensor) blocks
 uint32_t gn_chunk(uint64_t total_bytes);
 uint32_t gn_blocks(uint64_t n, int dtype, uint32_t chunk);
-// partial[b] of every block: sum of squares (ord 2), sum of |x| (1) or max |x| (0: infinity)
-void launch_grad_partials(const GradTable& t, int ord, double* partial, hipStream_t s);
+// partial[b] of every block: sum of squares (ord 2), sum of |x| (1) or max |x| (0: infinity); again: the tensors will be read
+// once more
+void launch_grad_partials(const GradTable& t, int ord, bool again, double* partial, hipStream_t s);
 // *norm from the n partials, and *coef = min(1, max_norm / (norm + 1e-6)) (coef may be null)
 void launch_grad_norm_final(const double* partial, uint32_t n, int ord, double max_norm, float* norm, double* coef,
                             hipStream_t s);

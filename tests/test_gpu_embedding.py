@@ -87,7 +87,7 @@ def test_lookup_and_gradient(hip_device, v, d, n, hot, dtype):
 def test_every_length_around_the_variants(hip_device):
     """Row counts, widths and lengths on either side of what chooses a variant; one token alone, and all alike."""
     from dogs_amd.embedding import embedding_lookup
-    for n in (1, 2, 63, 64, 65, 255, 256, 257, 1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 8193, 16385, 32769):
+    for n in (1, 2, 63, 64, 65, 255, 256, 257, 1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 8192, 8193, 16385, 32769):
         for v, d in ((n % 7 + 1, 24), (2000, 10)):
             for hot in (None, 1.1):
                 table, tokens, grad = _case(hip_device, v, d, n, torch.float32, torch.int64, seed=n, hot=hot)
