@@ -18,28 +18,25 @@ _WIDE = {torch.int64: 1, torch.int32: 0}
 
 def _lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float) -> torch.Tensor:
     v, d = table.shape
-    device = table.device
     out = table.new_empty((*tokens.shape, d))
-    with _lib.device_ctx(device):
-        _lib.check(_lib.load().dg_embedding_lookup(table.data_ptr(), _DTYPES[table.dtype], v, d, *table.stride(),
-                                                   tokens.data_ptr(), _WIDE[tokens.dtype], tokens.numel(), scale,
-                                                   out.data_ptr(), _lib.stream_of(device)))
+    _lib.launch(_lib.load().dg_embedding_lookup, table.get_device(), table.data_ptr(), _DTYPES[table.dtype], v, d,
+                table.stride(0), table.stride(1), tokens.data_ptr(), _WIDE[tokens.dtype], tokens.numel(), scale,
+                out.data_ptr())
     return out
 
 
 def _table_grad(ctx, g):
     tokens, = ctx.saved_tensors
     v, d, scale, padding = ctx.call
-    g = g.contiguous()
-    device, dtype, n = g.device, _DTYPES[g.dtype], tokens.numel()
+    if not g.is_contiguous():
+        g = g.contiguous()
+    dtype, n = _DTYPES[g.dtype], tokens.numel()
     L = _lib.load()
     dtable = g.new_empty((v, d))
     nbytes = L.dg_embedding_grad_scratch_bytes(v, d, n, dtype)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    with _lib.device_ctx(device):
-        _lib.check(L.dg_embedding_grad(g.data_ptr(), dtype, tokens.data_ptr(), _WIDE[tokens.dtype], n, v, d, scale, padding,
-                                       dtable.data_ptr(), scratch.data_ptr() if nbytes else None, nbytes,
-                                       _lib.stream_of(device)))
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=g.device) if nbytes else None
+    _lib.launch(L.dg_embedding_grad, g.get_device(), g.data_ptr(), dtype, tokens.data_ptr(), _WIDE[tokens.dtype], n, v, d,
+                scale, padding, dtable.data_ptr(), scratch.data_ptr() if nbytes else None, nbytes)
     return dtable, None, None, None
 
 
@@ -72,13 +69,13 @@ def embedding_lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1
     the stream: there such a token reads nothing, its row of the result is NaN, and it adds nothing to the gradient.
 
     The gradient is dense, in table's type, with every row written."""
-    _lib.require_device(table, "table")
-    if table.dim() != 2 or table.dtype not in _DTYPES:
+    if not table.is_cuda or table.dim() != 2 or table.dtype not in _DTYPES:
+        _lib.require_device(table, "table")
         raise RuntimeError(f"embedding_lookup: table must be [V, D] float32, float16 or bfloat16, got "
                            f"{tuple(table.shape)} {table.dtype}")
     if tokens.dtype not in _WIDE:
         raise RuntimeError(f"embedding_lookup: tokens must be int32 or int64, got {tokens.dtype}")
-    if tokens.device != table.device:
+    if tokens.get_device() != table.get_device():
         tokens = _to_device(tokens, table)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()

@@ -32,7 +32,7 @@ class _Table:
 
     def __init__(self, tensors: list, name: str, in_place: bool):
         self.device = tensors[0].device
-        index = tensors[0].get_device()
+        self.index = index = tensors[0].get_device()
         self.keep, self.copies = tensors, []
         for k, t in enumerate(tensors):
             if t.layout is not torch.strided or t.get_device() != index or index < 0 or t.dtype not in _DTYPES:
@@ -47,13 +47,9 @@ class _Table:
                         raise RuntimeError(f"{name}: a gradient's elements share memory: it cannot be scaled in place")
                     self.copies.append((t, self.keep[k]))
         self.n = len(tensors)
-        self.ptrs = array("Q", [t.data_ptr() for t in self.keep])
-        self.sizes = array("Q", [t.numel() for t in self.keep])
-        self.types = array("B", [_DTYPES[t.dtype] for t in self.keep])
-
-    @property
-    def args(self) -> tuple:
-        return (self.n, self.ptrs.buffer_info()[0], self.sizes.buffer_info()[0], self.types.buffer_info()[0])
+        self.lists = (array("Q", [t.data_ptr() for t in self.keep]), array("Q", [t.numel() for t in self.keep]),
+                      array("B", [_DTYPES[t.dtype] for t in self.keep]))
+        self.args = (self.n, *[a.buffer_info()[0] for a in self.lists])
 
     def write_back(self) -> None:
         for t, c in self.copies:
@@ -90,9 +86,7 @@ def grad_norm(tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: float =
     L = _lib.load()
     norm = torch.empty((), dtype=torch.float32, device=t.device)
     scratch, nbytes = _scratch(L, t)
-    with _lib.device_ctx(t.device):
-        _lib.check(L.dg_grad_norm(*t.args, order, 0.0, norm.data_ptr(), None, scratch.data_ptr(), nbytes,
-                                  _lib.stream_of(t.device)))
+    _lib.launch(L.dg_grad_norm, t.index, *t.args, order, 0.0, norm.data_ptr(), None, scratch.data_ptr(), nbytes)
     return norm
 
 
@@ -105,9 +99,7 @@ def clip_coefficient(tensors: list, max_norm: float) -> tuple:
     norm = torch.empty((), dtype=torch.float32, device=t.device)
     coef = torch.empty((), dtype=torch.float64, device=t.device)
     scratch, nbytes = _scratch(L, t)
-    with _lib.device_ctx(t.device):
-        _lib.check(L.dg_grad_norm(*t.args, 2, max_norm, norm.data_ptr(), coef.data_ptr(), scratch.data_ptr(), nbytes,
-                                  _lib.stream_of(t.device)))
+    _lib.launch(L.dg_grad_norm, t.index, *t.args, 2, max_norm, norm.data_ptr(), coef.data_ptr(), scratch.data_ptr(), nbytes)
     return norm, coef
 
 
@@ -128,17 +120,15 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
     L = _lib.load()
     norm = torch.empty((), dtype=torch.float32, device=t.device)
     scratch, nbytes = _scratch(L, t)
-    with _lib.device_ctx(t.device):
-        stream = _lib.stream_of(t.device)
-        if error_if_nonfinite:
-            coef = torch.empty((), dtype=torch.float64, device=t.device)
-            _lib.check(L.dg_grad_norm(*t.args, order, max_norm, norm.data_ptr(), coef.data_ptr(), scratch.data_ptr(),
-                                      nbytes, stream))
-            if not math.isfinite(float(norm)):
-                raise RuntimeError(f"clip_grad_norm_: the norm of the gradients is {float(norm)}")
-            _lib.check(L.dg_grad_scale(*t.args, coef.data_ptr(), stream))
-        else:
-            _lib.check(L.dg_clip_grad_norm(*t.args, order, max_norm, norm.data_ptr(), scratch.data_ptr(), nbytes, stream))
-        t.write_back()
+    if error_if_nonfinite:
+        coef = torch.empty((), dtype=torch.float64, device=t.device)
+        _lib.launch(L.dg_grad_norm, t.index, *t.args, order, max_norm, norm.data_ptr(), coef.data_ptr(), scratch.data_ptr(),
+                    nbytes)
+        if not math.isfinite(float(norm)):
+            raise RuntimeError(f"clip_grad_norm_: the norm of the gradients is {float(norm)}")
+        _lib.launch(L.dg_grad_scale, t.index, *t.args, coef.data_ptr())
+    else:
+        _lib.launch(L.dg_clip_grad_norm, t.index, *t.args, order, max_norm, norm.data_ptr(), scratch.data_ptr(), nbytes)
+    t.write_back()
     torch.autograd.graph.increment_version(grads)
     return norm
