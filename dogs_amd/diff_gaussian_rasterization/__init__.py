@@ -213,7 +213,7 @@ class SparseGaussianAdam(torch.optim.Adam):
 
         max_norm (optional): clip by the norm of all groups' gradients, every row's, as clip_grad_norm_ before the step
         would; the update multiplies the gradients by min(1, max_norm / (norm + 1e-6)) as it reads them, and they stay
-        as they are.  Returns the norm then, a 0-d float32 on the device (None without max_norm).  The penalty of prox
+        as they are (a norm that is NaN makes the visible rows NaN).  Returns the norm then, a 0-d float32 on the device (None without max_norm).  The penalty of prox
         is no part of the gradients here: the two together are refused."""
         if max_norm is not None and prox is not None:
             raise RuntimeError("step: max_norm does not see the penalty of prox: give one of the two")

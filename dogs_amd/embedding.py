@@ -68,7 +68,9 @@ def embedding_lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1
     Tokens outside [0, V) are an IndexError where tokens is on the host.  On the device reading them back would stall
     the stream: there such a token reads nothing, its row of the result is NaN, and it adds nothing to the gradient.
 
-    The gradient is dense, in table's type, with every row written."""
+    The gradient is dense, in table's type, with every row written.  Lookup and backward may be captured into a graph, the
+    backward only while no graph of the same table that was built outside the capture is alive (autograd would join
+    the two streams)."""
     if not table.is_cuda or table.dim() != 2 or table.dtype not in _DTYPES:
         _lib.require_device(table, "table")
         raise RuntimeError(f"embedding_lookup: table must be [V, D] float32, float16 or bfloat16, got "
@@ -79,6 +81,8 @@ def embedding_lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1
         tokens = _to_device(tokens, table)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
+    if isinstance(scale, torch.Tensor):
+        raise RuntimeError("embedding_lookup: scale must be a number (it gets no gradient)")
     padding = -1
     if padding_idx is not None:
         v = table.shape[0]

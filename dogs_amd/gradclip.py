@@ -77,7 +77,7 @@ def _scratch(L, t: _Table) -> tuple:
 
 def grad_norm(tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all elements of the tensors together (norm_type 2, 1 or inf), a 0-d float32 on their device.  float32,
-    float16 and bfloat16 may be mixed; no tensors: 0."""
+    float16 and bfloat16 may be mixed; no tensors: 0.  Not differentiable."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     order = _order("grad_norm", norm_type)
     if not tensors:
@@ -130,5 +130,5 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
     else:
         _lib.launch(L.dg_clip_grad_norm, t.index, *t.args, order, max_norm, norm.data_ptr(), scratch.data_ptr(), nbytes)
     t.write_back()
-    torch.autograd.graph.increment_version(grads)
+    torch.autograd.graph.increment_version([g for g in grads if not g.is_inference()])
     return norm

@@ -166,8 +166,9 @@ class AppearanceEmbedding(nn.Module):
 
     def _forward_batch(self, images: torch.Tensor, index: torch.Tensor, image_size: tuple) -> torch.Tensor:
         B, _, h, w = images.shape
-        if not isinstance(index, torch.Tensor) or tuple(index.shape) != (B,):
-            raise ValueError(f"AppearanceEmbedding: a batch of {B} images takes an int tensor of {B} view indices")
+        if B == 0 or not isinstance(index, torch.Tensor) or tuple(index.shape) != (B,):
+            raise ValueError(f"AppearanceEmbedding: a batch of {B} images takes an int tensor of {B} view indices, and one view "
+                             "at least")
         table = self.appearance_embedding
         if table.is_cuda:
             from .embedding import embedding_lookup

@@ -98,6 +98,20 @@ def test_every_length_around_the_variants(hip_device):
                 _check_grad(table.grad, grad, tokens, 0.5, v)
 
 
+@pytest.mark.parametrize("v,d,n,hot", [
+    (1, 3, 20000, None), (5_000_000, 2, 9000, 0.2), (2 ** 22, 3, 9000, None), (2 ** 22 - 1, 3, 9000, None),    # 1, 2, 3 sort passes
+    (1000, 3, 2 ** 18, 0.3), (1000, 3, 2 ** 18 + 1, 0.3), (3_000_000, 5, 300_000, 0.5), (3, 1, 600_000, None)])
+def test_long_lists(hip_device, v, d, n, hot):
+    """Lists on either side of what the wide-digit sort takes, tables of many rows, one row that all tokens share."""
+    from dogs_amd.embedding import embedding_lookup
+    table, tokens, grad = _case(hip_device, v, d, n, torch.bfloat16, torch.int64, seed=v % 97 + n, hot=hot)
+    table.requires_grad_(True)
+    out = embedding_lookup(table, tokens, scale=0.75, padding_idx=0 if v > 1 else None)
+    _check_lookup(out.detach(), table.detach(), tokens, 0.75)
+    out.backward(grad)
+    _check_grad(table.grad, grad, tokens, 0.75, v, 0 if v > 1 else None)
+
+
 @pytest.mark.parametrize("n", [9, 700, 30000])
 @pytest.mark.parametrize("padding", [0, 17, -1])
 def test_padding_row_gets_no_gradient(hip_device, padding, n):
@@ -276,6 +290,8 @@ def test_refusals(hip_device):
     for t, k in ((table.double(), tok), (table[0], tok), (table, tok.float()), (table, tok.bool()), (table.int(), tok)):
         with pytest.raises(RuntimeError):
             embedding_lookup(t, k)
+    with pytest.raises(RuntimeError):
+        embedding_lookup(table, tok, scale=torch.tensor(2.0, requires_grad=True))
     for p in (4, -5):
         with pytest.raises(IndexError):
             embedding_lookup(table, tok, padding_idx=p)
@@ -335,6 +351,8 @@ def test_appearance_batch_equals_the_single_views(hip_device):
     for bad in (3, [7, 2, 7], index[:2]):
         with pytest.raises(ValueError):
             net(images, bad, (100, 130))
+    with pytest.raises(ValueError):
+        net(images[:0], index[:0], (100, 130))
 
 
 def test_batched_clipped_step(hip_device):
