@@ -363,10 +363,10 @@ __device__ __forceinline__ float splat_power(float cx, float cy, float cz, float
     return fmaf(-0.5f, fmaf(cz * dy, dy, (cx * dx) * dx), -((cy * dx) * dy));
 }
 
-// Two pixels of one row (same dy) at once: ext_vector_type(2) arithmetic lowers to gfx950's packed
-// v_pk_{fma,mul,add}_f32.  On gfx950 a packed op issues in ~5 cycles for both halves whether or not it
-// depends on the previous instruction, while a dependent plain fp32 op costs ~5 cycles for one value
-// (tools/ubench_valu.hip) -- so the serial per-pixel compositing chain runs packed.
+// Two pixels of one row (same dy) at once, as ext_vector_type(2) arithmetic: two independent chains side by side.  A
+// dependent plain fp32 op costs ~5 cycles on gfx950, an independent one ~2.5 (tools/ubench_valu.hip), so the pair
+// costs what one pixel's serial compositing chain would.  The build leaves the packed instructions out (build.py): with
+// them the same 1080p step ran 1480 views/s, without 1466.
 typedef float v2f __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ v2f bc2(float x) { return (v2f){x, x}; }
 __device__ __forceinline__ v2f fma2(v2f a, v2f b, v2f c) { return __builtin_elementwise_fma(a, b, c); }
@@ -386,7 +386,7 @@ __device__ __forceinline__ v2f splat_power2(float A, float B, float C, v2f dx, f
 }
 
 // Four pixels per lane as {(c0, rA), (c0, rB), (c1, rA), (c1, rB)}: two columns c0, c0 + 8 of two rows
-// rA, rA + 8.  Each packed op's halves are independent rows, and lo + hi gives the two row sums.
+// rA, rA + 8.  The halves are independent rows, and lo + hi gives the two row sums.
 typedef float v4f __attribute__((ext_vector_type(4)));
 // Per-lane rows of a few floats (Gaussian parameters and gradients) are only 4-B aligned; one dwordx2/x3/x4 access per
 // row instead of one dword access per float: a wave's dword access touches up to 64 cache lines, and 45 of them per SH

@@ -80,12 +80,11 @@ __device__ __forceinline__ void stage_samples(const HeadArgs& a, int ry0, int rx
     }
 }
 
-// The weights are wave-uniform: every product reads them as scalar loads (SGPR operands of v_pk_fma_f32).  Staged in
+// The weights are wave-uniform: every product reads them as scalar loads (SGPR operands of the fmas).  Staged in
 // LDS as broadcast float4 rows they cost one LDS read per 6 FMAs and made the convolution loops LDS-issue-bound: head
 // forward 214 -> 169 us, backward 215 + 255 -> 182 + 225 us with the scalar form (gpurun_out/hw1, same box).
-// Two positions of a row at once: v_pk_fma_f32 with the weight broadcast to both halves (each half is the same fmaf
-// as the scalar form, so the bits do not change).  Left to itself the compiler paired output channels instead, and
-// spent a v_mov per weight building the pairs.
+// Two positions of a row at once, the weight broadcast to both halves (each half is the same fmaf as the scalar form, so
+// the bits do not change): two independent chains per weight read.
 typedef float f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f2 fma2(float w, f2 x, f2 acc) { return __builtin_elementwise_fma((f2)(w), x, acc); }
 

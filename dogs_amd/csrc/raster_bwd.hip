@@ -108,7 +108,7 @@ __device__ __forceinline__ void replay_splat(const RenderBwdArgs& a, const float
     for (int k = 0; k < 4; k++) dLda[k] = ok[k] ? dLda[k] : 0.0f;
     T = T * oma;
     // per-splat moments over the lane's 4 pixels; lo + hi of a v4 = the two row sums {row A, row B}.  A sum of
-    // products folds its hi half in with an fma (one packed op fewer per moment than product, product, add).
+    // products folds its hi half in with an fma (one op pair fewer per moment than product, product, add).
     const v4f t4 = G * dLda;
     const v4f tdx = t4 * dx;
     const v2f rt = lo2(t4) + hi2(t4);
@@ -157,7 +157,7 @@ __device__ __forceinline__ void replay_splat(const RenderBwdArgs& a, const float
 
 // Front-to-back replay.  Lane l owns pixels (l&7, l>>3) and (l&7 + 8, l>>3) of the tile's top half
 // (pair A = quadrants 0,1) and the same two of the bottom half (pair B = quadrants 2,3); each pair is
-// one row, evaluated with packed fp32.  Per 64-splat batch each lane stages its splat in wave-private
+// one row, a two-element vector.  Per 64-splat batch each lane stages its splat in wave-private
 // LDS with a 4-bit mask of the quadrants it can touch (quad_mask) that still have pixels before their
 // last contributor; the wave walks only splats with a non-empty mask and skips a pair whose two mask
 // bits are clear (wave-uniform branch).  Inactive (pixel, splat) pairs get alpha = 0, dL/dalpha = 0.

@@ -9,8 +9,8 @@
 //   k_emit         per prefix Gaussian: one (tile id, emission index, depth key) instance per kept tile
 //   tile binning   atomic counting sort by tile + per-tile sort into (depth bits, index) order (sortscan.hip):
 //                  the reference's (tile, depth bits, index) order, bit for bit
-//   k_render_fwd   one wave per 16x16 tile, 4 pixels per lane as two row pairs evaluated with packed fp32
-//                  (v_pk_*_f32); a 64-splat batch is staged in wave-private LDS and read back with broadcast
+//   k_render_fwd   one wave per 16x16 tile, 4 pixels per lane as two row pairs of two-element vectors; a
+//                  64-splat batch is staged in wave-private LDS and read back with broadcast
 //                  ds_read_b128; splats that cannot reach a quadrant pair skip it; wave-uniform early exit.
 #include <type_traits>
 #include <hip/hip_runtime.h>
@@ -994,7 +994,7 @@ __device__ __forceinline__ uint32_t bcast_u(uint32_t v, int lane) {
 
 // renderCUDA (forward.cu:349-501) restructured for wave64: one wave per 16x16 tile, 4 pixels per lane.
 // Lane l owns pixels (l&7, l>>3) and (l&7 + 8, l>>3) of the top half (pair A = quadrants 0,1) and the
-// same two of the bottom half (pair B = quadrants 2,3); each pair is one row, evaluated with packed fp32.
+// same two of the bottom half (pair B = quadrants 2,3); each pair is one row, a two-element vector.
 // Each 64-splat batch is gathered one splat per lane (one 32-B splat record + colour), tested against
 // the four quadrants with the reference's own max-contribution rect test (quad_mask), and staged in
 // wave-private LDS; the wave then walks only splats that reach a quadrant (s_ff1 over a 64-bit ballot),
