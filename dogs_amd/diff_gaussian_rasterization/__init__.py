@@ -249,9 +249,10 @@ def _clip(groups, visibility, N, max_norm):
     if visibility.numel() != N:
         raise RuntimeError(f"step: visibility has {visibility.numel()} entries for {N} rows")
     index = visibility.get_device()
-    for group in groups:
-        n = group[0].numel()
-        if any(t.numel() != n or t.get_device() != index for t in group[:4]) or (n % N if N else n):
+    for p, g, m, v, _, _ in groups:
+        n = p.numel()
+        if (g.numel() != n or m.numel() != n or v.numel() != n or (n % N if N else n) or p.get_device() != index
+                or g.get_device() != index or m.get_device() != index or v.get_device() != index):
             raise RuntimeError(f"step: a group's tensors are not {N} rows each on {visibility.device}")
     if not groups:
         return torch.zeros((), device=visibility.device), None
