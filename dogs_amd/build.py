@@ -36,7 +36,7 @@ def _stale(obj: str, src: str) -> bool:
         return True
     t = os.path.getmtime(obj)
     deps = [src] + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
-    deps.append(os.path.join(HERE, "..", "include", "dogs_hip.h"))
+    deps += [os.path.join(HERE, "..", "include", "dogs_hip.h"), os.path.abspath(__file__)]   # and the flags above
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 

@@ -1,7 +1,7 @@
 // embedding.hip -- embedding lookup and its gradient (embedding.h).
 //
 //   lookup    Y[i] = s E[t_i];  a token outside [0, V) gives a row of NaN
-//   gradient  dE[v] = s sum_{i: t_i = v} G[i], summed in the order of i;  0 for the padding token and for v without one
+//   gradient  dE[v] = s sum_{i: t_i = v} G[i], in an order that the tokens set;  0 for the padding token and for v without one
 #include <hip/hip_runtime.h>
 
 #include "dtypes.h"

@@ -143,8 +143,8 @@ class AppearanceEmbedding(nn.Module):
         """image: [3, h, w] (the 32x-downsampled target); index: the view's row of the embedding table;
         image_size: (H, W) of the render.  Returns the [3, H, W] mask.
 
-        A batch of B views of one size: image [B, 3, h, w] and index an int tensor [B] (on the device or the host);
-        returns [B, 3, H, W].  The codes are then one embedding_lookup, and the table's gradient its sorted sums: a view
+        A batch of B views of one size: image [B, 3, h, w] and index an int tensor [B] (on the device or the host, as
+        embedding_lookup takes it); returns [B, 3, H, W].  The codes are then one embedding_lookup, and the table's gradient its sorted sums: a view
         that is in the batch twice adds both."""
         if image.dim() == 4:
             return self._forward_batch(image, index, image_size)
