@@ -411,6 +411,9 @@ def adam_update_groups(groups, visible, N, b1=0.9, b2=0.999, stats=None, prox=No
     if vis.dtype != torch.bool:
         vis = vis.bool()
     dev = vis.device
+    if grad_coef is not None and (grad_coef.dtype != torch.float64 or grad_coef.device != dev or grad_coef.numel() != 1):
+        raise RuntimeError(f"grad_coef must be one float64 on {dev}, got {grad_coef.numel()} {grad_coef.dtype} on "
+                           f"{grad_coef.device}")
     keep = [vis]
     arr = (_lib.DgAdamGroup * max(1, min(8, len(groups))))()
     st = None

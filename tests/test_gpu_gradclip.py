@@ -339,6 +339,12 @@ def test_clipped_step_refusals(hip_device):
         opt.step(torch.ones(n + 1, dtype=torch.bool, device=hip_device), n + 1, max_norm=1.0)
     with pytest.raises(RuntimeError):
         opt.step(vis, n, max_norm=-1.0)
+    from diff_gaussian_rasterization import _C
+    group = [(ps[0], ps[0].grad, opt.state[ps[0]]["exp_avg"], opt.state[ps[0]]["exp_avg_sq"], 1e-3, 1e-15)]
+    for coef in (torch.ones((), device=hip_device), torch.ones(2, dtype=torch.float64, device=hip_device),
+                 torch.ones((), dtype=torch.float64)):
+        with pytest.raises(RuntimeError):
+            _C.adam_update_groups(group, vis, n, grad_coef=coef)
     opt.state[ps[0]]["exp_avg"] = torch.zeros((n - 1, 3), device=hip_device)
     with pytest.raises(RuntimeError):
         opt.step(vis, n, max_norm=1.0)
