@@ -164,7 +164,7 @@ template <typename L> struct Stretch {
     float *head, *tail;      // the block's partials, D floats each (null: neither end is open)
 };
 
-constexpr int WALK = 8;
+constexpr int WALK = 8;   // rows in flight; four are as fast, twelve or sixteen take half as long again (registers)
 
 // THREADS threads; s_part: LDS of THREADS * 2 * W floats
 template <typename T, bool PAST, int THREADS, typename L>
@@ -260,8 +260,8 @@ __device__ __forceinline__ void sum_stretch(const LookupGradArgs& a, const Stret
 // A block owns `rows` (a power of two, up to 256) rows of the table and one slab of columns.  It looks through all tokens,
 // each wave through a contiguous part of them, ranks those of its rows (stable counting sort by row, in LDS), and sums.
 // The list is 64 IT NW entries long at most; LDS and the tokens that a lane looks at go with it (256 tokens of 64 fp32 take 6 us
-// in the kernel for 1024, 9 in that for 4096).  1024 blocks are aimed at: twice as many cost 0 to 25 % (each looks through
-// all tokens), half as many 0 to 25 % in small tables, and save 3 % in large ones.  Stored through the caches
+// in the kernel for 1024, 9 in that for 4096).  1024 blocks are aimed at: twice as many cost up to a third (each looks through
+// all tokens), half as many up to an eighth in small tables, and save 5 % in large ones.  Stored through the caches
 // whatever the size: past them a table of 50021 x 1023 fp16 took 4 to 13 us more, one of 131072 x 2048 bf16 no less.
 template <typename T, int NW, int IT>
 __global__ void __launch_bounds__(NW * 64) k_grad_small(LookupGradArgs a, int lpr, uint32_t rows, int row_bits, uint32_t slabs) {
@@ -580,6 +580,13 @@ uint32_t slabs_of(uint32_t D, int dtype, int lpr) {
 // for 16384 tokens fills a CU alone and was slower (62 us at 8191).
 constexpr uint32_t SMALL_N = 8192;
 
+// ... unless its few blocks would each add up a long list: a table of few rows, where a group of lanes has over 160 tokens to
+// walk.  8000 tokens of 1024 bf16 in 2 rows: 100 us in one launch, 24 sorted; in 16 rows 21 and 23.
+bool one_launch(const LookupGradArgs& a, int dtype) {
+    const uint32_t threads = a.n <= 4096 ? 256u : 512u;
+    return a.n <= SMALL_N && a.n <= 160ull * a.V * (threads / lanes_per_row(a.D, dtype));
+}
+
 SumPlan plan_of(const LookupGradArgs& a, int dtype) {
     SumPlan p = {};
     p.lpr = lanes_per_row(a.D, dtype);
@@ -650,14 +657,13 @@ void launch_embedding_lookup(const LookupArgs& a, int dtype, hipStream_t s) {
 }
 
 size_t embedding_grad_scratch_bytes(uint32_t V, uint32_t D, uint32_t n, int dtype) {
-    if (n <= SMALL_N) return 0;
     LookupGradArgs a = {};
     a.V = V; a.D = D; a.n = n;
-    return scratch_of(a, plan_of(a, dtype)).bytes;
+    return one_launch(a, dtype) ? 0 : scratch_of(a, plan_of(a, dtype)).bytes;
 }
 
 void launch_embedding_grad(const LookupGradArgs& a, int dtype, void* scratch, hipStream_t s) {
-    if (a.n <= SMALL_N) {
+    if (one_launch(a, dtype)) {
         if (dtype == 0) grad_small<float>(a, dtype, s);
         else if (dtype == 1) grad_small<_Float16>(a, dtype, s);
         else grad_small<__bf16>(a, dtype, s);

@@ -99,6 +99,7 @@ def test_every_length_around_the_variants(hip_device):
 
 
 @pytest.mark.parametrize("v,d,n,hot", [
+    (1, 600, 3000, None), (2, 300, 8000, None), (3, 517, 7000, 0.5), (1, 2, 8192, None),      # few rows with long lists
     (1, 3, 20000, None), (5_000_000, 2, 9000, 0.2), (2 ** 22, 3, 9000, None), (2 ** 22 - 1, 3, 9000, None),    # 1, 2, 3 sort passes
     (1000, 3, 2 ** 18, 0.3), (1000, 3, 2 ** 18 + 1, 0.3), (3_000_000, 5, 300_000, 0.5), (3, 1, 600_000, None)])
 def test_long_lists(hip_device, v, d, n, hot):
