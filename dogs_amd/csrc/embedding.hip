@@ -580,11 +580,33 @@ uint32_t slabs_of(uint32_t D, int dtype, int lpr) {
 // for 16384 tokens fills a CU alone and was slower (62 us at 8191).
 constexpr uint32_t SMALL_N = 8192;
 
-// ... unless its few blocks would each add up a long list: a table of few rows, where a group of lanes has over 160 tokens to
-// walk.  8000 tokens of 1024 bf16 in 2 rows: 100 us in one launch, 24 sorted; in 16 rows 21 and 23.
+// The one-launch kernel's blocks: `rows` rows of the table (a power of two, 2^bits) and a slab of half a wave's 16-byte pieces each.
+// (A whole wave's: as fast where the tokens are spread, but one token that is 40 % of 8192 takes 111 us instead of 77 in
+// 50000 rows of 1024 bf16; a quarter's: 55 instead of 41 where they are spread.)
+struct SmallPlan {
+    int lpr, bits;
+    uint32_t rows, slabs, threads;
+    uint64_t blocks;
+};
+SmallPlan small_plan(const LookupGradArgs& a, int dtype) {
+    SmallPlan p = {};
+    p.lpr = lanes_per_row(a.D, dtype);
+    if (p.lpr > 32) p.lpr = 32;
+    p.slabs = slabs_of(a.D, dtype, p.lpr);
+    p.rows = 1;
+    while (p.rows < 256 && (uint64_t)((a.V + p.rows - 1) / p.rows) * p.slabs > 1024) { p.rows <<= 1; p.bits++; }
+    p.blocks = ((uint64_t)a.V + p.rows - 1) / p.rows * p.slabs;
+    p.threads = a.n <= 4096 ? 256u : 512u;
+    return p;
+}
+
+// ... unless its few blocks would each add up a long list (a table of few rows, where a group of lanes has over 160 tokens to
+// walk: 8000 tokens of 1024 bf16 in 2 rows take 100 us in one launch, 24 sorted), or its many blocks would each look through
+// many tokens (8192 of 2048 bf16 in 131072 rows: 160 us, sorted 131).
 bool one_launch(const LookupGradArgs& a, int dtype) {
-    const uint32_t threads = a.n <= 4096 ? 256u : 512u;
-    return a.n <= SMALL_N && a.n <= 160ull * a.V * (threads / lanes_per_row(a.D, dtype));
+    if (a.n > SMALL_N) return false;
+    const SmallPlan p = small_plan(a, dtype);
+    return a.n <= 160ull * a.V * (p.threads / p.lpr) && a.n * p.blocks <= (1ull << 24);
 }
 
 SumPlan plan_of(const LookupGradArgs& a, int dtype) {
@@ -616,15 +638,10 @@ GradScratch scratch_of(const LookupGradArgs& a, const SumPlan& p) {
 
 template <typename T>
 void grad_small(const LookupGradArgs& a, int dtype, hipStream_t s) {
-    const int lpr = lanes_per_row(a.D, dtype);
-    const uint32_t slabs = slabs_of(a.D, dtype, lpr);
-    uint32_t rows = 1;
-    int bits = 0;
-    while (rows < 256 && (uint64_t)((a.V + rows - 1) / rows) * slabs > 1024) { rows <<= 1; bits++; }
-    const uint64_t blocks = (uint64_t)((a.V + rows - 1) / rows) * slabs;
-    if (a.n <= 1024) k_grad_small<T, 4, 4><<<(uint32_t)blocks, 256, 0, s>>>(a, lpr, rows, bits, slabs);
-    else if (a.n <= 4096) k_grad_small<T, 4, 16><<<(uint32_t)blocks, 256, 0, s>>>(a, lpr, rows, bits, slabs);
-    else k_grad_small<T, 8, 16><<<(uint32_t)blocks, 512, 0, s>>>(a, lpr, rows, bits, slabs);
+    const SmallPlan p = small_plan(a, dtype);
+    if (a.n <= 1024) k_grad_small<T, 4, 4><<<(uint32_t)p.blocks, 256, 0, s>>>(a, p.lpr, p.rows, p.bits, p.slabs);
+    else if (a.n <= 4096) k_grad_small<T, 4, 16><<<(uint32_t)p.blocks, 256, 0, s>>>(a, p.lpr, p.rows, p.bits, p.slabs);
+    else k_grad_small<T, 8, 16><<<(uint32_t)p.blocks, 512, 0, s>>>(a, p.lpr, p.rows, p.bits, p.slabs);
 }
 
 bool past_caches(const LookupGradArgs& a, int dtype) {
