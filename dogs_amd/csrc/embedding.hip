@@ -602,11 +602,11 @@ SmallPlan small_plan(const LookupGradArgs& a, int dtype) {
 
 // ... unless its few blocks would each add up a long list (a table of few rows, where a group of lanes has over 160 tokens to
 // walk: 8000 tokens of 1024 bf16 in 2 rows take 100 us in one launch, 24 sorted), or its many blocks would each look through
-// many tokens (8192 of 2048 bf16 in 131072 rows: 160 us, sorted 131).
+// many tokens (8192 of 2048 bf16 in 131072 rows: 160 us, sorted 131; up to 1024 tokens a lane looks through four at most).
 bool one_launch(const LookupGradArgs& a, int dtype) {
     if (a.n > SMALL_N) return false;
     const SmallPlan p = small_plan(a, dtype);
-    return a.n <= 160ull * a.V * (p.threads / p.lpr) && a.n * p.blocks <= (1ull << 24);
+    return a.n <= 160ull * a.V * (p.threads / p.lpr) && (a.n <= 1024 || a.n * p.blocks <= (1ull << 24));
 }
 
 SumPlan plan_of(const LookupGradArgs& a, int dtype) {

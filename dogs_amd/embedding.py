@@ -33,7 +33,7 @@ def _table_grad(ctx, g):
     dtype, n = _DTYPES[g.dtype], tokens.numel()
     L = _lib.load()
     dtable = g.new_empty((v, d))
-    nbytes = L.dg_embedding_grad_scratch_bytes(v, d, n, dtype)
+    nbytes = L.dg_embedding_grad_scratch_bytes(v, d, n, dtype) if n > 1024 else 0     # few tokens need none
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=g.device) if nbytes else None
     _lib.launch(L.dg_embedding_grad, g.get_device(), g.data_ptr(), dtype, tokens.data_ptr(), _WIDE[tokens.dtype], n, v, d,
                 scale, padding, dtable.data_ptr(), scratch.data_ptr() if nbytes else None, nbytes)

@@ -245,7 +245,7 @@ int dg_embedding_lookup(const void* table, int dtype, uint64_t V, uint32_t D, in
 /* Its gradient for the table: dtable [V][D] (every element is written) = scale * sum of the rows i of grad [n][D] with
  * tokens[i] == v, for every v != padding (-1: none); sums in 32 bits in an order that only the tokens set, without
  * atomics.  Tokens outside [0, V) add nothing.  scratch of dg_embedding_grad_scratch_bytes(V, D, n, dtype) bytes
- * (0 where few tokens need none: it may be NULL then). */
+ * (0 up to 1024 tokens and for some longer lists: it may be NULL then). */
 size_t dg_embedding_grad_scratch_bytes(uint64_t V, uint32_t D, uint64_t n, int dtype);
 int dg_embedding_grad(const void* grad, int dtype, const void* tokens, int wide, uint64_t n, uint64_t V, uint32_t D,
                       float scale, int64_t padding, void* dtable, void* scratch, size_t scratch_bytes,

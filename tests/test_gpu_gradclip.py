@@ -349,3 +349,64 @@ def test_clipped_step_refusals(hip_device):
     with pytest.raises(RuntimeError):
         opt.step(vis, n, max_norm=1.0)
     assert all(torch.equal(p.detach(), b) for p, b in zip(ps, before))
+
+
+def test_clipped_step_in_a_graph(hip_device):
+    """A captured clipped step replays as the eager one: same parameters, moments and norm after each of several replays, with
+    other gradients and eager work between them."""
+    n = 3001
+    ps, opt, vis = _scene(hip_device, n, 11)
+    qs, eager, _ = _scene(hip_device, n, 11)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):          # recorded, not run
+        norm = opt.step(vis, n, max_norm=0.05)
+    for k in range(4):
+        for p, q in zip(ps, qs):
+            fresh = torch.randn(p.shape, generator=torch.Generator().manual_seed(100 + k)).to(hip_device) * 10.0 ** -(k + 2)
+            p.grad.copy_(fresh)
+            q.grad = fresh
+        graph.replay()
+        want = eager.step(vis, n, max_norm=0.05)
+        torch.cuda.synchronize()
+        assert torch.equal(norm, want)
+        for p, q in zip(ps, qs):
+            assert torch.equal(p, q)
+            assert all(torch.equal(opt.state[p][s], eager.state[q][s]) for s in ("exp_avg", "exp_avg_sq"))
+
+
+def test_two_threads_at_once(hip_device):
+    """Two host threads, each with a stream of its own: lookups with gradients and clipping do not see each other."""
+    import threading
+
+    from dogs_amd.embedding import embedding_lookup
+    from dogs_amd.gradclip import clip_grad_norm_
+    wrong = []
+
+    def work(seed, n):
+        try:
+            g = torch.Generator().manual_seed(seed)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                table = torch.randint(-4, 5, (300, 20), generator=g).float().to(hip_device).requires_grad_(True)
+                for _ in range(20):
+                    tokens = torch.randint(0, 300, (n,), generator=g)
+                    grad = torch.randint(-3, 4, (n, 20), generator=g).float()
+                    out = embedding_lookup(table, tokens.to(hip_device))
+                    out.backward(grad.to(hip_device))
+                    want = torch.zeros(300, 20).index_add_(0, tokens, grad)      # whole numbers: exact in any order
+                    total = math.sqrt(float((want.double() ** 2).sum()))
+                    got = table.grad.cpu()
+                    norm = float(clip_grad_norm_(table, total / 2))
+                    clipped = want.double() * (total / 2 / (total + 1e-6))
+                    if not (torch.equal(got, want) and abs(norm - total) <= 2 * U * total
+                            and bool(((table.grad.cpu().double() - clipped).abs() <= 4 * U * clipped.abs()).all())):
+                        wrong.append((seed, n))
+                    table.grad = None
+        except Exception as e:  # noqa: BLE001 - reported by the assertion below
+            wrong.append(repr(e))
+    threads = [threading.Thread(target=work, args=a) for a in ((1, 500), (2, 9000))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

@@ -43,6 +43,10 @@ def test_embedding_entry_refusals(lib):
         return lib.dg_embedding_grad(g, dtype, tokens, 1, n, v, d, 1.0, -1, out, scratch, nbytes, None)
     need = lib.dg_embedding_grad_scratch_bytes(4, 4, 20000, 0)
     assert need > 0
+    for v in (1, 2, 1000, 1 << 20, (1 << 31) - 1):      # the Python side does not ask up to 1024 tokens
+        for d in (1, 64, 4096, (1 << 23) - 1):
+            for dtype in (0, 1, 2):
+                assert lib.dg_embedding_grad_scratch_bytes(v, d, 1024, dtype) == 0
     for kw in ({"dtype": 3}, {"v": 1 << 31}, {"n": 1 << 31}, {"d": 1 << 23}, {"g": None}, {"tokens": None}, {"out": None},
                {"n": 20000, "scratch": None}, {"n": 20000, "nbytes": need - 1}):
         assert grad(**kw) != 0, kw
