@@ -1213,7 +1213,8 @@ int dg_embedding_lookup(const void* table, int dtype, uint64_t V, uint32_t D, in
 }
 
 size_t dg_embedding_grad_scratch_bytes(uint64_t V, uint32_t D, uint64_t n, int dtype) {
-    if (V >= (1ull << 31) || n >= (1ull << 31) || dtype < 0 || dtype > 2) return 0;
+    // an empty table launches nothing, and sizes outside the limits are refused by the call itself
+    if (V == 0 || D == 0 || V >= (1ull << 31) || n >= (1ull << 31) || D >= (1u << 23) || dtype < 0 || dtype > 2) return 0;
     return gs::embedding_grad_scratch_bytes((uint32_t)V, D, (uint32_t)n, dtype);
 }
 

@@ -317,6 +317,16 @@ def test_empty(hip_device):
     assert bare.grad.shape == (0, 6)
 
 
+@pytest.mark.parametrize("n", [2, 1025, 9000])
+def test_table_without_columns(hip_device, n):
+    from dogs_amd.embedding import embedding_lookup
+    flat = torch.empty((4, 0), device=hip_device, requires_grad=True)
+    out = embedding_lookup(flat, torch.zeros(n, dtype=torch.int64, device=hip_device))
+    assert out.shape == (n, 0)
+    out.sum().backward()
+    assert flat.grad.shape == (4, 0)
+
+
 def _network(dev, views):
     from dogs_amd.masks import AppearanceEmbedding
     torch.manual_seed(0)

@@ -54,6 +54,16 @@ def test_embedding_entry_refusals(lib):
     assert lib.dg_embedding_grad_scratch_bytes(1 << 31, 4, 2, 0) == 0
 
 
+def test_scratch_of_empty_and_refused_sizes(lib):
+    """A table without rows or columns needs no scratch, however long the list (the row's bytes divide nothing), and sizes
+    that the gradient refuses are not priced."""
+    for n in (1, 1024, 1025, 8192, 8193, 9000, 300_000, (1 << 31) - 1):
+        for dtype in (0, 1, 2):
+            for v, d in ((4, 0), (0, 4), (0, 0), ((1 << 31) - 1, 0), (4, 1 << 23), (4, (1 << 32) - 1)):
+                assert lib.dg_embedding_grad_scratch_bytes(v, d, n, dtype) == 0, (v, d, n, dtype)
+    assert lib.dg_embedding_grad(16, 0, 16, 1, 9000, 4, 0, 1.0, -1, 16, None, 0, None) == 0
+
+
 def test_gradient_entry_refusals(lib):
     def args(ptrs, sizes, types):
         keep = array("Q", ptrs), array("Q", sizes), array("B", types)
