@@ -13,6 +13,7 @@ import threading
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "libdogs_hip.so")
@@ -386,6 +387,19 @@ def device_ctx(device: torch.device):
     if device.index is None or device.index == _GET_DEVICE():
         return _SAME_DEVICE
     return torch.cuda.device(device)
+
+
+_IS_TRACING = getattr(torch._C, "_is_tracing", None) or torch.jit.is_tracing     # 0.1 us instead of 0.4 us
+
+
+def refuse_unrecorded(name: str, tensors) -> None:
+    """Error for what would record or differentiate a call that fills its result through a raw pointer outside an autograd
+    function: torch.jit.trace would keep the empty result alone, and a forward-mode tangent would be lost."""
+    if _IS_TRACING():
+        raise RuntimeError(f"{name} cannot be traced: its kernels leave nothing for torch.jit.trace to record")
+    # the level first: unpacking every gradient of a network would cost more than the launch
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def launch(fn, index: int, *args) -> None:

@@ -26,6 +26,7 @@ def _lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float) -> torch.Te
 
 
 def _table_grad(ctx, g):
+    _lib.refuse_unrecorded("embedding_lookup's gradient", (g,))
     tokens, = ctx.saved_tensors
     v, d, scale, padding = ctx.call
     if not g.is_contiguous():
@@ -68,6 +69,8 @@ def embedding_lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1
     Tokens outside [0, V) are an IndexError where tokens is on the host.  On the device reading them back would stall
     the stream: there such a token reads nothing, its row of the result is NaN, and it adds nothing to the gradient.
 
+    Forward-mode tangents, of the table or of the result's gradient, and torch.jit.trace are refused.
+
     The gradient is dense, in table's type, with every row written.  Lookup and backward may be captured into a graph, the
     backward only while no graph of the same table that was built outside the capture is alive (autograd would join
     the two streams)."""
@@ -75,6 +78,7 @@ def embedding_lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1
         _lib.require_device(table, "table")
         raise RuntimeError(f"embedding_lookup: table must be [V, D] float32, float16 or bfloat16, got "
                            f"{tuple(table.shape)} {table.dtype}")
+    _lib.refuse_unrecorded("embedding_lookup", (table,))
     if tokens.dtype not in _WIDE:
         raise RuntimeError(f"embedding_lookup: tokens must be int32 or int64, got {tokens.dtype}")
     if tokens.get_device() != table.get_device():

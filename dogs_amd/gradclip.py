@@ -31,6 +31,7 @@ class _Table:
     """The tensors of a call as the library takes them; keeps what it points at."""
 
     def __init__(self, tensors: list, name: str, in_place: bool):
+        _lib.refuse_unrecorded(name, tensors)
         self.device = tensors[0].device
         self.index = index = tensors[0].get_device()
         self.keep, self.copies = tensors, []
@@ -77,7 +78,8 @@ def _scratch(L, t: _Table) -> tuple:
 
 def grad_norm(tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all elements of the tensors together (norm_type 2, 1 or inf), a 0-d float32 on their device.  float32,
-    float16 and bfloat16 may be mixed; no tensors: 0.  Not differentiable."""
+    float16 and bfloat16 may be mixed; no tensors: 0.  Not differentiable: forward-mode tangents are refused, and so is
+    torch.jit.trace."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     order = _order("grad_norm", norm_type)
     if not tensors:

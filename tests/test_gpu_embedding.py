@@ -274,6 +274,40 @@ def test_second_derivative_is_refused(hip_device):
         dt.sum().backward()
 
 
+@pytest.mark.parametrize("learns", [False, True])
+def test_forward_mode_is_refused(hip_device, learns):
+    """A dual table, and a dual gradient of the result (forward over reverse): an error, not a derivative of zero."""
+    import torch.autograd.forward_ad as fw
+
+    from dogs_amd.embedding import embedding_lookup
+    table = torch.randn((5, 4), device=hip_device, requires_grad=learns)
+    tokens = torch.tensor([0, 3, 3], device=hip_device)
+    with fw.dual_level():
+        dual = fw.make_dual(table, torch.ones_like(table))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            embedding_lookup(dual, tokens)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            embedding_lookup(dual, tokens)
+        out = embedding_lookup(table, tokens)      # what carries no tangent goes on
+        assert torch.equal(out, table[tokens])
+        if learns:
+            g = torch.ones((3, 4), device=hip_device)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, table, fw.make_dual(g, g))
+            dt, = torch.autograd.grad(embedding_lookup(table, tokens), table, g)
+            assert torch.equal(dt[:, 0].cpu(), torch.tensor([1.0, 0.0, 0.0, 2.0, 0.0]))
+
+
+@pytest.mark.parametrize("learns", [False, True])
+def test_tracing_is_refused(hip_device, learns):
+    from dogs_amd.embedding import embedding_lookup
+    table = torch.randn((5, 4), device=hip_device, requires_grad=learns)
+    tokens = torch.tensor([0, 3, 3], device=hip_device)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda e: embedding_lookup(e, tokens), (table,))
+    assert torch.equal(embedding_lookup(table, tokens), table[tokens])
+
+
 def test_tokens_changed_before_the_backward_are_noticed(hip_device):
     from dogs_amd.embedding import embedding_lookup
     table = torch.randn((5, 4), device=hip_device, requires_grad=True)

@@ -209,6 +209,30 @@ def test_empty_and_refusals(hip_device):
     assert torch.equal(p.grad, torch.ones(3, device=hip_device))
 
 
+def test_forward_mode_and_tracing_are_refused(hip_device):
+    import torch.autograd.forward_ad as fw
+
+    from dogs_amd.gradclip import clip_coefficient, clip_grad_norm_, grad_norm
+    x = torch.ones(9, device=hip_device)
+    p = torch.nn.Parameter(torch.zeros(9, device=hip_device))
+    with fw.dual_level():
+        p.grad = fw.make_dual(x, x)
+        for call in (lambda: grad_norm([x, p.grad]), lambda: clip_grad_norm_(p, 1.0), lambda: clip_coefficient([p.grad], 1.0)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert float(grad_norm(x)) == 3.0
+        p.grad = None
+    p.grad = x
+
+    def clipped(g):
+        p.grad = g
+        return clip_grad_norm_(p, 1.0)
+    for f in (lambda g: grad_norm([g]), clipped):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(f, (torch.ones(9, device=hip_device),))
+    assert bool((x == 1.0).all())
+
+
 def test_in_place_change_is_seen_by_autograd(hip_device):
     from dogs_amd.gradclip import clip_grad_norm_
     p, = _params([torch.ones(8, device=hip_device)])
