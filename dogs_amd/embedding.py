@@ -29,6 +29,8 @@ def _table_grad(ctx, g):
     _lib.refuse_unrecorded("embedding_lookup's gradient", (g,))
     tokens, = ctx.saved_tensors
     v, d, scale, padding = ctx.call
+    if g.is_neg():
+        g = g.resolve_neg()
     if not g.is_contiguous():
         g = g.contiguous()
     dtype, n = _DTYPES[g.dtype], tokens.numel()
@@ -79,6 +81,8 @@ def embedding_lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1
         raise RuntimeError(f"embedding_lookup: table must be [V, D] float32, float16 or bfloat16, got "
                            f"{tuple(table.shape)} {table.dtype}")
     _lib.refuse_unrecorded("embedding_lookup", (table,))
+    if table.is_neg():      # a view of a conjugate's imaginary part: its memory holds the other sign
+        table = table.resolve_neg()
     if tokens.dtype not in _WIDE:
         raise RuntimeError(f"embedding_lookup: tokens must be int32 or int64, got {tokens.dtype}")
     if tokens.get_device() != table.get_device():

@@ -190,6 +190,29 @@ def test_strides(hip_device):
     assert torch.equal(slim.grad.cpu(), want)
 
 
+def test_negated_views(hip_device):
+    """Views whose memory holds the other sign (a conjugate's imaginary part): as a table, contiguous or strided, one that
+    learns, and as the result's gradient."""
+    from dogs_amd.embedding import embedding_lookup
+    g = torch.Generator().manual_seed(8)
+    tokens = torch.tensor([1, 1, 5], device=hip_device)
+    z = torch.complex(torch.randn((6, 8), generator=g), torch.randn((6, 8), generator=g)).to(hip_device)
+    for view, want in ((z.conj().imag, -z.imag), (torch._neg_view(z.real.contiguous()), -z.real)):
+        assert view.is_neg()
+        assert torch.equal(embedding_lookup(view, tokens), want[tokens])
+        leaf = view.detach().requires_grad_(True)
+        out = embedding_lookup(leaf, tokens)
+        assert torch.equal(out, want[tokens])
+        out[0].sum().backward()
+        assert torch.equal(leaf.grad[:, 0].cpu(), torch.tensor([0.0, 1.0, 0.0, 0.0, 0.0, 0.0]))
+    table = torch.randn((6, 8), generator=g).to(hip_device).requires_grad_(True)
+    out = embedding_lookup(table, tokens)
+    up = torch.randn((3, 8), generator=g).to(hip_device)
+    a, = torch.autograd.grad(out, table, torch._neg_view(up), retain_graph=True)
+    b, = torch.autograd.grad(out, table, -up)
+    assert torch.equal(a, b)
+
+
 def test_gradient_against_differences(hip_device):
     """The lookup is linear: on small whole numbers and a power of two as scale every product and sum here is exact, so a
     difference of the loss equals the gradient's product with the step to the last bit."""
