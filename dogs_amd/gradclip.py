@@ -7,6 +7,7 @@ import math
 from array import array
 from typing import Iterable
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -27,6 +28,62 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _extent(t: torch.Tensor) -> tuple:
+    """The bytes between t's first and last element."""
+    first = t.data_ptr()
+    return first, first + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _as_numpy(t: torch.Tensor) -> np.ndarray:
+    """t's addresses as an array that is never read, for np.shares_memory."""
+    class Layout:
+        __array_interface__ = {"version": 3, "data": (t.data_ptr(), True), "typestr": f"<u{t.element_size()}",
+                               "shape": tuple(t.shape), "strides": tuple(st * t.element_size() for st in t.stride())}
+    return np.asarray(Layout())
+
+
+def _shares_memory(a: np.ndarray, b: np.ndarray) -> bool:
+    try:
+        return np.shares_memory(a, b, max_work=10_000)      # exact; the work is bounded
+    except np.exceptions.TooHardError:
+        return True                                          # too interleaved to tell apart
+
+
+def _repeats(t: torch.Tensor) -> bool:
+    """Whether two of t's elements are the same memory."""
+    reach = 0
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st <= reach:
+            break
+        reach += st * (n - 1)
+    else:
+        return False       # each stride steps over all that the smaller ones reach
+    a = _as_numpy(t)
+    for k in range(t.dim()):     # two elements whose first difference is in dimension k
+        if t.shape[k] > 1 and _shares_memory(a[(0,) * k + (slice(0, 1),)], a[(0,) * k + (slice(1, None),)]):
+            return True
+    return False
+
+
+def _check_apart(tensors: list, gapped: list, name: str) -> None:
+    """Error where a gapped tensor shares memory with itself or another: the library sees its copy only.  (Tensors
+    without gaps it compares itself.)"""
+    for k in gapped:
+        if _repeats(tensors[k]):
+            raise RuntimeError(f"{name}: a gradient's elements share memory: it cannot be scaled in place")
+    gapped, reaching = set(gapped), []
+    for first, end, k in sorted((*_extent(t), k) for k, t in enumerate(tensors) if t.numel()):
+        reaching = [r for r in reaching if r[0] > first]
+        a = _as_numpy(tensors[k]) if reaching or k in gapped else None
+        for r in reaching:
+            if k in gapped or r[1] in gapped:
+                if r[2] is None:
+                    r[2] = _as_numpy(tensors[r[1]])
+                if _shares_memory(a, r[2]):
+                    raise RuntimeError(f"{name}: gradients to scale overlap in memory")
+        reaching.append([end, k, a])
+
+
 class _Table:
     """The tensors of a call as the library takes them; keeps what it points at."""
 
@@ -34,7 +91,7 @@ class _Table:
         _lib.refuse_unrecorded(name, tensors)
         self.device = tensors[0].device
         self.index = index = tensors[0].get_device()
-        self.keep, self.copies = tensors, []
+        self.keep, gapped = tensors, []
         for k, t in enumerate(tensors):
             if t.layout is not torch.strided or t.get_device() != index or index < 0 or t.dtype not in _DTYPES:
                 raise RuntimeError(f"{name}: gradients must be dense float32, float16 or bfloat16 tensors on one HIP "
@@ -43,10 +100,10 @@ class _Table:
                 if self.keep is tensors:
                     self.keep = list(tensors)
                 self.keep[k] = t.contiguous()
-                if in_place:
-                    if any(st == 0 and sz > 1 for st, sz in zip(t.stride(), t.shape)):
-                        raise RuntimeError(f"{name}: a gradient's elements share memory: it cannot be scaled in place")
-                    self.copies.append((t, self.keep[k]))
+                gapped.append(k)
+        if in_place and gapped:
+            _check_apart(tensors, gapped, name)
+        self.copies = [(tensors[k], self.keep[k]) for k in gapped]
         self.n = len(tensors)
         self.lists = (array("Q", [t.data_ptr() for t in self.keep]), array("Q", [t.numel() for t in self.keep]),
                       array("B", [_DTYPES[t.dtype] for t in self.keep]))

@@ -177,6 +177,41 @@ def test_shared_gradients(hip_device):
     assert bool((flat == 3.0).all())
 
 
+@pytest.mark.parametrize("which", ["two with gaps", "one with gaps over a dense one", "the same one twice", "in itself", "types",
+                                   "far apart"])
+def test_shared_gradients_with_gaps(hip_device, which):
+    """Gradients with gaps are scaled through copies: shared elements are found in the gradients themselves."""
+    from dogs_amd.gradclip import clip_grad_norm_, grad_norm
+    half = torch.full((60, 50), 3.0, device=hip_device)
+    bits = half.view(torch.bfloat16)
+    grads = {"two with gaps": [half[3:50, 7:40], half[3:50, 8:41]],
+             "one with gaps over a dense one": [half[10:20], half[3:50, 7:40]],
+             "the same one twice": [half[:, 2:9]] * 2,
+             "in itself": [half.as_strided((4, 4), (1, 2))],
+             "types": [half[:, 2:9], bits[:, 17:30]],
+             "far apart": [half[:, :9], half[40:, 12:20], half[1:, 8:12]]}[which]
+    before = half.clone()
+    for fail in (False, True):
+        with pytest.raises(RuntimeError, match="share memory" if which == "in itself" else "overlap"):
+            clip_grad_norm_(_params(grads), 1.0, error_if_nonfinite=fail)
+    assert torch.equal(half, before)
+    assert math.isfinite(float(grad_norm(grads[:1])))      # a norm alone may read an element twice
+
+
+def test_interleaved_gradients(hip_device):
+    """Columns of one buffer, as six gradients: their extents cross, their elements do not."""
+    from dogs_amd.gradclip import clip_grad_norm_
+    rows = torch.randn((3001, 59), generator=torch.Generator().manual_seed(3)).to(hip_device)
+    old, grads, at = rows.clone(), [], 0
+    for w in (3, 3, 45, 1, 3, 4):
+        grads.append(rows[:, at:at + w])
+        at += w
+    n = _norm([old])
+    assert abs(float(clip_grad_norm_(_params(grads), n / 2)) - n) <= 2 * U * n
+    want = old.double() * (n / 2 / (n + 1e-6))
+    assert bool(((rows.double() - want).abs() <= 4 * U * want.abs() + TINY[torch.float32]).all())
+
+
 def test_past_32_bit_sizes(hip_device):
     from dogs_amd.gradclip import clip_grad_norm_, grad_norm
     n = 2 ** 32 + 12345

@@ -90,6 +90,40 @@ def test_gradient_entry_refusals(lib):
     assert lib.dg_grad_norm(2, None, None, None, 2, 1.0, 256, None, 256, need, None) != 0
 
 
+def test_shared_memory_is_found():
+    """The comparison of gradients with gaps, against the sets of the bytes that they cover."""
+    import itertools
+    import random
+
+    from dogs_amd import gradclip as G
+    rng = random.Random(1)
+    buffer = torch.zeros(400)
+
+    def view():
+        shape = [rng.randint(1, 5) for _ in range(rng.randint(1, 3))]
+        strides = [rng.choice((0, 1, 2, 3, 4, 5, 7, 10, 12, 20)) for _ in shape]
+        return buffer.view(rng.choice((torch.float32, torch.bfloat16))).as_strided(shape, strides, rng.randint(0, 40))
+
+    def covered(t):
+        e = t.element_size()
+        return [t.data_ptr() + e * sum(i * s for i, s in zip(at, t.stride())) + b
+                for at in itertools.product(*map(range, t.shape)) for b in range(e)]
+    found = [0, 0]
+    for _ in range(2000):
+        views = [view() for _ in range(rng.randint(1, 4))]
+        gapped = [k for k, t in enumerate(views) if not G._dense(t)]
+        cover = [covered(t) for t in views]
+        want = any(len(set(cover[k])) < len(cover[k]) for k in gapped) or any(
+            set(cover[i]) & set(cover[j]) for i in range(len(views)) for j in range(i) if i in gapped or j in gapped)
+        found[want] += 1
+        if want:
+            with pytest.raises(RuntimeError):
+                G._check_apart(views, gapped, "clip")
+        else:
+            G._check_apart(views, gapped, "clip")
+    assert min(found) > 100
+
+
 def test_appearance_batch_on_the_host():
     """The batched module on the CPU equals its single views; a view that is there twice adds both gradients."""
     from dogs_amd.masks import AppearanceEmbedding
