@@ -120,10 +120,19 @@ def pre_phase_iterations(cfg: ADMMRunConfig) -> int:
     return 0 if d <= 0 else int(math.ceil(d / k)) * k
 
 
+def _refuse_clipping(cfg: ADMMRunConfig, start_iteration: int) -> None:
+    """GSTrainConfig.max_grad_norm is the pre-phase's alone: the ADMM rounds' step adds the penalty's gradient as it reads
+    the loss's, and a norm of both is not formed.  A run that goes on into such rounds has to do without it."""
+    if cfg.gs.max_grad_norm > 0.0 and start_iteration < cfg.gs.max_iterations:
+        raise ValueError(f"max_grad_norm = {cfg.gs.max_grad_norm}: the ADMM rounds do not clip (set it to 0, or max_iterations to "
+                         f"the pre-phase's {start_iteration})")
+
+
 def block_train_config(cfg: ADMMRunConfig, pre: GaussianSplatTrainer, start_iteration: int,
                        sh_degree: int) -> TrainConfig:
     """The re-created worker's setup (setup_training_params / setup_optimizer): the same optimizer.lr and loss keys,
     the same spatial_lr_scale (same cameras), continuing at the master's iteration (update_iteration)."""
+    _refuse_clipping(cfg, start_iteration)
     gs = cfg.gs
     return TrainConfig(position_init=gs.position_init, position_final=gs.position_final,
                        position_delay_mult=gs.position_delay_mult,
@@ -138,6 +147,8 @@ def run(cfg: ADMMRunConfig, scene: BlockScene, group=None, device=None, seed: in
         max_rounds: int | None = None) -> RankRun:
     """This rank's whole run (scene.block = its rank in `group`).  max_rounds caps the ADMM rounds (None: until
     max_iterations)."""
+    n_pre = pre_phase_iterations(cfg)
+    _refuse_clipping(cfg, n_pre)      # now, not after the pre-phase
     rank = dist.get_rank(group)
     if scene.block != rank:
         raise RuntimeError(f"rank {rank} was given block {scene.block}: one block per rank, in rank order")
@@ -145,7 +156,6 @@ def run(cfg: ADMMRunConfig, scene: BlockScene, group=None, device=None, seed: in
     secs = {}
     t0 = time.perf_counter()
     pre = pre_phase_trainer(cfg, scene, dev, seed)
-    n_pre = pre_phase_iterations(cfg)
     while pre.iteration < n_pre:            # train_every_x_interval chunks (the master's RPC rounds)
         pre.train(cfg.admm.consensus_interval)
     pre.sync()
@@ -188,10 +198,11 @@ class SequentialRun:
 def run_sequential(cfg: ADMMRunConfig, scenes: list, device, seed: int = 0, kernels=None,
                    max_rounds: int | None = None) -> SequentialRun:
     """The same run for every block on one device, one block after another (scenes[b].block == b)."""
+    n_pre = pre_phase_iterations(cfg)
+    _refuse_clipping(cfg, n_pre)
     dev = torch.device(device)
     secs = {}
     t0 = time.perf_counter()
-    n_pre = pre_phase_iterations(cfg)
     pres = []
     for sc in scenes:
         pre = pre_phase_trainer(cfg, sc, dev, seed)

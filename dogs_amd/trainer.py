@@ -35,7 +35,8 @@ Options of the reference configs (GSTrainConfig.from_reference reads them from t
 
 Clipping (no reference key): max_grad_norm > 0 clips the six tensors' gradients by their common norm inside
 SparseGaussianAdam.step; every iteration then takes the autograd route, because the native step folds the activations'
-backward into its update and never holds the gradients that the norm is of.  mask_max_grad_norm > 0 clips the appearance
+backward into its update and never holds the gradients that the norm is of.  A distributed run (admm_run) whose ADMM
+rounds would follow refuses it: they do not clip.  mask_max_grad_norm > 0 clips the appearance
 embedding's with clip_grad_norm_, on both routes.  last_grad_norm is the last iteration's norm before clipping.
 """
 from __future__ import annotations

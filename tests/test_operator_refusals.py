@@ -124,6 +124,26 @@ def test_shared_memory_is_found():
     assert min(found) > 100
 
 
+def test_admm_run_refuses_clipping():
+    """The ADMM rounds do not clip: a run that asks for it and has such rounds is refused before it trains anything."""
+    from types import SimpleNamespace
+
+    from dogs_amd.admm_run import ADMMRunConfig, block_train_config, pre_phase_iterations, run, run_sequential
+    from dogs_amd.trainer import GSTrainConfig
+    cfg = ADMMRunConfig(gs=GSTrainConfig(max_iterations=1000, densify_end_iter=300, max_grad_norm=0.1))
+    start, pre = pre_phase_iterations(cfg), SimpleNamespace(spatial_lr_scale=5.0)
+    assert 300 <= start < 1000
+    for call in (lambda: run(cfg, None), lambda: run_sequential(cfg, [], "cuda:0"),
+                 lambda: block_train_config(cfg, pre, start, 3)):
+        with pytest.raises(ValueError, match="max_grad_norm"):
+            call()
+    cfg.gs.max_iterations = start                    # no round follows the pre-phase
+    assert block_train_config(cfg, pre, start, 3).start_iteration == start
+    cfg.gs.max_iterations, cfg.gs.max_grad_norm = 1000, 0.0
+    cfg.gs.mask_max_grad_norm = 0.1                  # the rounds have no appearance mask
+    assert block_train_config(cfg, pre, start, 3).sh_degree == 3
+
+
 def test_appearance_batch_on_the_host():
     """The batched module on the CPU equals its single views; a view that is there twice adds both gradients."""
     from dogs_amd.masks import AppearanceEmbedding
