@@ -37,7 +37,9 @@ Clipping (no reference key): max_grad_norm > 0 clips the six tensors' gradients 
 SparseGaussianAdam.step; every iteration then takes the autograd route, because the native step folds the activations'
 backward into its update and never holds the gradients that the norm is of.  A distributed run (admm_run) whose ADMM
 rounds would follow refuses it: they do not clip.  mask_max_grad_norm > 0 clips the appearance
-embedding's with clip_grad_norm_, on both routes.  last_grad_norm is the last iteration's norm before clipping.
+embedding's with clip_grad_norm_, on both routes.  last_grad_norm is the norm of the last iteration's six gradients, before
+clipping; a tensor that densification, a reset or a prune replaces in the iteration takes no step in it and is no part of
+the norm that the others are clipped by.
 """
 from __future__ import annotations
 
@@ -415,6 +417,10 @@ class GaussianSplatTrainer:
         loss = loss + c.lambda_scale * row_prod(out["scaling"]).mean()
         loss.backward()
         self.last_loss = loss.detach()
+        if c.max_grad_norm > 0.0 and ev:    # the events replace tensors, whose gradients go with them
+            from .gradclip import grad_norm
+            grads = [g["params"][0].grad for g in self.optimizer.param_groups]
+            self.last_grad_norm = grad_norm([g for g in grads if g is not None])
         replaced = False
         with torch.no_grad():
             if self.iteration < c.densify_end_iter:
@@ -434,7 +440,9 @@ class GaussianSplatTrainer:
                 m.prune_gaussians_with_opt((c.prune_decay ** i) * c.prune_percent, v, self.optimizer)
                 replaced = True
         if c.max_grad_norm > 0.0:
-            self.last_grad_norm = self.optimizer.step(radii > 0, radii.shape[0], max_norm=c.max_grad_norm)
+            norm = self.optimizer.step(radii > 0, radii.shape[0], max_norm=c.max_grad_norm)
+            if not ev:
+                self.last_grad_norm = norm
         else:
             self.optimizer.step(radii > 0, radii.shape[0])
         self.optimizer.zero_grad(set_to_none=True)

@@ -39,6 +39,26 @@ def test_a_limit_out_of_reach_changes_nothing(hip_device):
     assert plain.last_grad_norm is None and clipped.last_grad_norm.shape == ()
 
 
+def test_the_recorded_norm_is_of_all_six_gradients(hip_device, monkeypatch):
+    """Also in an iteration whose densification, reset or prune replaces tensors: not 0, and not of the rest alone."""
+    from dogs_amd import trainer as T
+    kw = dict(densify_start_iter=2, densification_interval=4, opacity_reset_interval=7, prune_iterations=(10,),
+              max_iterations=12)
+    tr = _run(hip_device, _cfg(max_grad_norm=1e9, **kw), 0)
+    backward, want = torch.Tensor.backward, []
+
+    def noting(self, *a, **k):
+        backward(self, *a, **k)
+        grads = [g["params"][0].grad for g in tr.optimizer.param_groups]
+        want.append(math.sqrt(sum(float((g.double() ** 2).sum()) for g in grads)))
+    monkeypatch.setattr(T.torch.Tensor, "backward", noting)
+    for _ in range(12):
+        tr.train_iteration()
+        assert abs(float(tr.last_grad_norm) - want[-1]) <= 2 * U * want[-1] and want[-1] > 0.0
+    assert len(want) == 12
+    assert {e for lg in tr.logs for e in lg.events} == {"densify", "reset_opacity", "prune"}
+
+
 def test_a_limit_within_reach_scales_the_step(hip_device):
     kw = dict(densify_start_iter=10 ** 6, opacity_reset_interval=10 ** 6, prune_iterations=())
     free = _run(hip_device, _cfg(max_grad_norm=1e9, **kw), 1)
