@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(NW * 64) k_grad_small(LookupGradArgs a, int lp
     }
     __syncthreads();
     const Cols<T, false> c = cols_of<T, false>(slab, lpr, t & (lpr - 1), a.D);
-    // rows without a token: the last wave's start of row r, advanced past its tokens, is where row r + 1 begins
+    // rows without a token: the first wave's start of a row is the row's, and where row r + 1 begins row r ends
     for (uint32_t r = t / lpr; r < nrows; r += NW * 64 / lpr) {
         const uint32_t end = r + 1 < 256 ? s_hist[0][r + 1] : total;
         if (s_hist[0][r] == end) c.store((T*)a.dtable + (uint64_t)(v0 + r) * a.D, typename Vec<T>::type{});

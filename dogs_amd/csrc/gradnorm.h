@@ -9,7 +9,8 @@ namespace gs {
 // tensors of one launch; their table travels in the kernel arguments (2.7 KB of the 4 KB), so no host memory has to
 // outlive the call and a captured graph holds its own copy
 constexpr int GN_MAX = 128;
-// at most this many blocks (= double partials) over all launches of a call
+// at most this many blocks (= double partials) over all launches of a call, and one more per tensor: each ends in a
+// block of its own
 constexpr uint32_t GN_MAX_BLOCKS = 4096;
 constexpr uint32_t GN_MIN_CHUNK = 16384;  // bytes of a block
 
@@ -22,7 +23,7 @@ struct GradTable {
     uint32_t chunk;               // bytes of a block
 };
 
-// the chunk size at which the tensors take at most GN_MAX_BLOCKS (+ one per tensor) blocks
+// the chunk size for that
 uint32_t gn_chunk(uint64_t total_bytes);
 uint32_t gn_blocks(uint64_t n, int dtype, uint32_t chunk);
 // partial[b] of every block: sum of squares (ord 2), sum of |x| (1) or max |x| (0: infinity); again: the tensors will be read

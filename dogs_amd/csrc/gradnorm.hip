@@ -129,7 +129,9 @@ __device__ __forceinline__ void chunk_scale(T* __restrict__ p, uint64_t n, doubl
 __global__ void __launch_bounds__(GN_THREADS) k_grad_scale(GradTable t, const double* __restrict__ coef) {
     const double c = *coef;
     if (c == 1.0) return;  // x * 1 is x
-    const uint32_t b = gridDim.x - 1 - blockIdx.x;  // from the back: the end is what the norm left in the caches
+    // from the back: the end is what the norm left in the caches.  (The launches of more than GN_MAX tensors go front to
+    // back: in reverse 300 tensors of 240 MB took 151 us with their norm instead of 150, of 600 MB 397 instead of 394.)
+    const uint32_t b = gridDim.x - 1 - blockIdx.x;
     const int k = tensor_of(t, b);
     const uint64_t per = t.dtype[k] == 0 ? t.chunk / 4 : t.chunk / 2;
     const uint64_t e0 = (uint64_t)(b - t.start[k]) * per;

@@ -166,10 +166,11 @@ def clip_coefficient(tensors: list, max_norm: float) -> tuple:
 def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_: scales the parameters' gradients in place by min(1, max_norm / (norm + 1e-6)) of
-    the norm of them all (norm_type 2, 1 or inf) and returns that norm, a 0-d float32 on their device.  Gradients within
-    max_norm are not written at all.  Parameters without a gradient are left out, and one that is given twice
-    counts once; gradients that share memory are refused.  A norm that is NaN makes every gradient NaN, an infinite one
-    makes them 0 (NaN where they were infinite), unless error_if_nonfinite, which reads the norm back and raises."""
+    the norm of them all (norm_type 2, 1 or inf) and returns that norm, a 0-d float32 on their device.  With a
+    coefficient of 1 gradients keep every bit (and are not written, but for those with gaps, which are scaled in a copy and
+    copied back).  Parameters without a gradient are left out, and one that is given twice counts once; gradients that share
+    memory are refused.  A norm that is NaN makes every gradient NaN, an infinite one makes them 0 (NaN where they were
+    infinite, and all of them with an infinite max_norm), unless error_if_nonfinite, which reads the norm back and raises."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     order, max_norm = _order("clip_grad_norm_", norm_type), _max_norm("clip_grad_norm_", max_norm)
     grads = [p.grad for p in dict.fromkeys(parameters) if p.grad is not None]

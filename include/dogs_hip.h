@@ -262,7 +262,7 @@ int dg_grad_norm(int n_tensors, const void* const* tensors, const uint64_t* nume
  * must not overlap (an error). */
 int dg_grad_scale(int n_tensors, void* const* tensors, const uint64_t* numel, const uint8_t* dtype, const double* coef,
                   dg_stream_t stream);
-/* Both: *norm as dg_grad_norm and, when it exceeds max_norm, the tensors scaled down to it. */
+/* Both: *norm as dg_grad_norm and, where the coefficient is not 1, the tensors times it. */
 int dg_clip_grad_norm(int n_tensors, void* const* tensors, const uint64_t* numel, const uint8_t* dtype, int ord,
                       double max_norm, float* norm, void* scratch, size_t scratch_bytes, dg_stream_t stream);
 
