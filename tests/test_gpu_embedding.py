@@ -113,6 +113,41 @@ def test_long_lists(hip_device, v, d, n, hot):
     _check_grad(table.grad, grad, tokens, 0.75, v, 0 if v > 1 else None)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("v,d,n,hot", [
+    (2, 300, 8000, None), (2 ** 22, 3, 9000, 0.2), (1000, 3, 2 ** 18, 0.3), (700, 37, 2 ** 18 + 1, 0.3), (200_000, 65, 300_000, None)])
+def test_long_lists_of_other_types(hip_device, v, d, n, hot, dtype):
+    from dogs_amd.embedding import embedding_lookup
+    table, tokens, grad = _case(hip_device, v, d, n, dtype, torch.int32, seed=v % 89 + n, hot=hot)
+    table.requires_grad_(True)
+    out = embedding_lookup(table, tokens, scale=0.25, padding_idx=1)
+    _check_lookup(out.detach(), table.detach(), tokens, 0.25)
+    out.backward(grad)
+    _check_grad(table.grad, grad, tokens, 0.25, v, 1)
+
+
+def test_long_list_in_a_graph(hip_device):
+    """The sort of more than 2^18 tokens, captured: several replays with other tokens and eager work between them."""
+    from dogs_amd.embedding import embedding_lookup
+    v, n = 3000, 2 ** 18 + 77
+    table, tokens, grad = _case(hip_device, v, 9, n, torch.float32, torch.int64, seed=12)
+    table.requires_grad_(True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dt, = torch.autograd.grad(embedding_lookup(table, tokens), table, grad)
+    for k in range(3):
+        g = torch.Generator().manual_seed(60 + k)
+        tokens.copy_(torch.randint(0, v >> k, (n,), generator=g))
+        grad.copy_(torch.randn((n, 9), generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = dt.clone()
+        _check_grad(got, grad, tokens, 1.0, v)
+        eager, = torch.autograd.grad(embedding_lookup(table, tokens), table, grad)
+        assert torch.equal(got, eager)
+
+
 @pytest.mark.parametrize("n", [9, 700, 30000])
 @pytest.mark.parametrize("padding", [0, 17, -1])
 def test_padding_row_gets_no_gradient(hip_device, padding, n):
