@@ -60,7 +60,8 @@ __device__ __forceinline__ int tensor_of(const GradTable& t, uint32_t b) {
 
 // AGAIN: the tensors are read once more after this (the scaling, the clipped update): they pass through the caches then,
 // which keep up to 256 MB for it.  Otherwise the loads pass by them: 1e6 x 59 floats in 34 us (6.9 TB/s) instead of 40,
-// while the update after it took 259 us instead of 244.
+// while the update after it took 259 us instead of 244.  (Above 256 MB they evict each other: 403 MB of bf16 that were just
+// written 96 us instead of 65; the rule goes by use alone.)
 template <int ORD, bool AGAIN, typename T>
 __device__ __forceinline__ double chunk_norm(const T* __restrict__ p, uint64_t n) {
     typedef typename Vec<T>::type V;
